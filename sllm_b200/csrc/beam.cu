@@ -1,0 +1,512 @@
+// Beam search on the device: the best continuations of every search over its beams and the whole vocabulary, and what of them goes on or is finished.
+// The reference decodes one sequence by sampling alone (runtime/sampler.py:36-88); it has no search.
+//
+// Candidates.  With m_b the largest logit of beam b, the continuation of beam b by token v scores
+//   s(b, v) = score_b + ((x_bv - m_b) - log sum_u exp(x_bu - m_b)),
+// and the `keep` largest of a search are wanted, in order: s descending, then the beam, then the logit descending, then the token.  Within a beam s grows with the
+// logit, so a beam's own best are those of the largest logits, and no candidate of the search lies outside the `keep` best of its beam:
+//   beam_rows_kernel    a part of a row a block: the part's maximum, its sum of exponentials and its `keep` largest logits, from one pass over the logits;
+//   beam_merge_kernel   a block a search, a warp a beam: the beam's parts joined, then the beams.
+// Exponentials are expf of float32 differences, exact as the logits are; their sums over a row's threads and parts, the logarithm and s are float64 (continuations
+// of different beams are compared with each other; of one beam by their logits alone).  s is rounded to float32 once, when it is stored.
+#include "common.cuh"
+
+namespace sllm {
+
+constexpr int BEAM_THREADS = 256, BEAM_KEEP = 128, BEAM_MAX = 32;
+constexpr int BEAM_LOADS = 4;                                   // 16-byte loads a thread and batch
+constexpr uint32_t BEAM_MINUS_INFINITY = 0x007fffffu;           // the key of minus infinity: what is not above it offers nothing
+
+// Keys: the logit's bits so that unsigned order is float order, then the token turned around, so that of equal logits the first is the largest key.  0: no key.
+__device__ __forceinline__ uint32_t beam_order(float f) {
+  const uint32_t u = __float_as_uint(f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float beam_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+__device__ __forceinline__ unsigned long long beam_key(float f, int token) { return (unsigned long long)beam_order(f) << 32 | ~(uint32_t)token; }
+__device__ __forceinline__ unsigned long long order_double(double v) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double double_of(unsigned long long k) {
+  return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
+}
+__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (unsigned long long)hi << 32 | lo;
+}
+
+// a part of a row: the sum of exp(logit - max), and its largest logit
+struct BeamPart {
+  double sum;
+  float max;
+};
+
+template <typename T> struct BeamLoad;
+template <> struct BeamLoad<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& raw, float* x) {
+    x[0] = __uint_as_float(raw.x);
+    x[1] = __uint_as_float(raw.y);
+    x[2] = __uint_as_float(raw.z);
+    x[3] = __uint_as_float(raw.w);
+  }
+};
+template <> struct BeamLoad<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& raw, float* x) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+
+// The list of keys that may belong to the best: what a batch can add (see beam_rows_kernel) beside the `keep` it already holds, and the other half of a
+// filter's ping-pong, which is at most half as long.
+constexpr int BEAM_LIST = BEAM_KEEP * BEAM_LOADS * 8 + BEAM_KEEP, BEAM_OTHER = BEAM_LIST / 2 + BEAM_KEEP;
+
+struct BeamShared {
+  unsigned long long list[BEAM_LIST], other[BEAM_OTHER];
+  unsigned long long group[BEAM_THREADS];
+  unsigned long long bound;
+  int n;
+  float red_m[BEAM_THREADS / 32];
+  double red_s[BEAM_THREADS / 32];
+};
+
+// The keep-th largest of the groups' largest keys, known to all threads: `keep` keys at least are no smaller.  0 where fewer than `keep` groups have a key.
+// `mine`: this thread's largest; a group is 1 << log2_lanes threads side by side.
+__device__ unsigned long long beam_group_bound(unsigned long long mine, int log2_lanes, int keep, BeamShared& sh) {
+  for (int o = 1; o < (1 << log2_lanes); o <<= 1) {
+    const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, o);
+    mine = mine > other ? mine : other;
+  }
+  const int groups = BEAM_THREADS >> log2_lanes;
+  if ((threadIdx.x & ((1 << log2_lanes) - 1)) == 0) sh.group[threadIdx.x >> log2_lanes] = mine;
+  if (threadIdx.x == 0) sh.bound = 0;
+  __syncthreads();
+  if (threadIdx.x < groups) {
+    const unsigned long long me = sh.group[threadIdx.x];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < groups; ++j) rank += sh.group[j] > me || (sh.group[j] == me && j < (int)threadIdx.x);
+    if (rank == keep - 1) sh.bound = me;
+  }
+  __syncthreads();
+  const unsigned long long b = sh.bound;
+  __syncthreads();
+  return b;
+}
+
+// The keys sh.list[0, sh.n) become their `keep` largest, sorted; returns how many there are.  Filters by the groups' bound until 256 at most are left (each pass leaves at most
+// (keep - 1) groups' keys and one, under half of them), then every key finds its place.
+__device__ int beam_compact(int keep, int log2_lanes, BeamShared& sh) {
+  __syncthreads();
+  int n = sh.n;
+  unsigned long long *from = sh.list, *to = sh.other;
+  while (n > BEAM_THREADS) {
+    unsigned long long best = 0;
+    for (int i = threadIdx.x; i < n; i += BEAM_THREADS) best = best > from[i] ? best : from[i];
+    const unsigned long long b = beam_group_bound(best, log2_lanes, keep, sh);
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += BEAM_THREADS)
+      if (from[i] >= b) to[atomicAdd(&sh.n, 1)] = from[i];
+    __syncthreads();
+    n = sh.n;
+    unsigned long long* t = from;
+    from = to;
+    to = t;
+    __syncthreads();
+  }
+  const unsigned long long me = (int)threadIdx.x < n ? from[threadIdx.x] : 0;
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) rank += from[j] > me;
+  __syncthreads();
+  if ((int)threadIdx.x < n && rank < keep) sh.list[rank] = me;
+  n = n < keep ? n : keep;
+  if (threadIdx.x == 0) sh.n = n;
+  __syncthreads();
+  return n;
+}
+
+// One part of one row: blockIdx.x = row * splits + part.  What bounds it: reading the logits once.  A batch is BEAM_LOADS 16-byte loads a thread, all in flight
+// together; of a batch only keys that reach the bound, a key that `keep` others are known to reach, enter the list.
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const T* logits, int V, int keep, int log2_lanes, int splits, int part_vecs, BeamPart* parts, unsigned long long* keys) {
+  constexpr int N = BeamLoad<T>::N, VALUES = BEAM_LOADS * N;
+  extern __shared__ __align__(16) unsigned char beam_smem[];
+  BeamShared& sh = *reinterpret_cast<BeamShared*>(beam_smem);
+  const int row = blockIdx.x / splits, part = blockIdx.x - row * splits;
+  const T* x_row = logits + (size_t)row * V;
+  // Pieces of 16 bytes of tokens.  Which thread takes which tokens goes by their numbers and not by where the row lies, so that equal rows give equal sums; a row that does not begin
+  // on 16 bytes is read an element at a time (from L1 but for the first of a piece).
+  const int pieces = (V + N - 1) / N;
+  const bool aligned = (reinterpret_cast<uintptr_t>(x_row) & 15) == 0;
+  const int v0 = part * part_vecs, v1 = min(v0 + part_vecs, pieces);
+  if (threadIdx.x == 0) sh.n = 0;
+  unsigned long long bound = (unsigned long long)(BEAM_MINUS_INFINITY + 1) << 32;
+  int n_most = 0;                                  // the list's length at most, the same in all threads
+  float m = -INFINITY, s = 0.f;
+  __syncthreads();
+  pdl_wait();
+  for (int vb = v0; vb < v1; vb += BEAM_LOADS * BEAM_THREADS) {
+    float x[VALUES];
+#pragma unroll
+    for (int u = 0; u < BEAM_LOADS; ++u) {
+      const int v = vb + u * BEAM_THREADS + threadIdx.x, first = v * N;
+      if (aligned && v < v1 && first + N <= V) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(x_row + first);
+        BeamLoad<T>::unpack(raw, x + u * N);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[u * N + i] = v < v1 && first + i < V ? to_f32(x_row[first + i]) : -INFINITY;
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VALUES; ++i) {
+      x[i] = x[i] == x[i] ? x[i] + 0.0f : -INFINITY;          // not a number: no candidate; minus zero is zero
+      top = fmaxf(top, x[i]);
+    }
+    if (top > m) {
+      s *= expf(m - top);                          // (minus infinity first: times zero)
+      m = top;
+    }
+    if (m > -INFINITY) {
+      float p0 = 0.f, p1 = 0.f;
+      if (m < INFINITY) {
+#pragma unroll
+        for (int i = 0; i < VALUES; i += 2) {
+          p0 += expf(x[i] - m);
+          p1 += expf(x[i + 1] - m);
+        }
+      } else {                                     // all of the mass lies on the infinite ones
+        for (int i = 0; i < VALUES; ++i) p0 += x[i] == m ? 1.f : 0.f;
+      }
+      s += p0 + p1;
+    }
+    // the list
+    const bool reaches = beam_order(top) >= (uint32_t)(bound >> 32) && top > -INFINITY;
+    const int flagged = __syncthreads_count(reaches);
+    if (flagged == 0) continue;
+    if (n_most + flagged * VALUES > BEAM_LIST) {
+      n_most = sh.n;                               // (nobody adds before the next barrier)
+      __syncthreads();
+      if (n_most + flagged * VALUES > BEAM_LIST) {
+        if (n_most > 0) {
+          n_most = beam_compact(keep, log2_lanes, sh);
+          if (n_most == keep) bound = bound > sh.list[keep - 1] ? bound : sh.list[keep - 1];
+        }
+        // of this batch: keys from the keep-th largest of the groups' largest on, which are those of fewer than `keep` groups and one more
+        unsigned long long best = 0;
+#pragma unroll
+        for (int u = 0; u < BEAM_LOADS; ++u)
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const unsigned long long k = beam_key(x[u * N + i], (vb + u * BEAM_THREADS + (int)threadIdx.x) * N + i);
+            if (x[u * N + i] > -INFINITY && k > best) best = k;
+          }
+        const unsigned long long b = beam_group_bound(best, log2_lanes, keep, sh);
+        bound = bound > b ? bound : b;
+        n_most = BEAM_LIST;                        // (looked up again when it matters)
+      } else {
+        n_most += flagged * VALUES;
+      }
+    } else {
+      n_most += flagged * VALUES;
+    }
+    if (reaches) {
+#pragma unroll
+      for (int u = 0; u < BEAM_LOADS; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (!(x[u * N + i] > -INFINITY)) continue;
+          const unsigned long long k = beam_key(x[u * N + i], (vb + u * BEAM_THREADS + (int)threadIdx.x) * N + i);
+          if (k >= bound) sh.list[atomicAdd(&sh.n, 1)] = k;
+        }
+    }
+  }
+  pdl_launch_dependents();
+  // the part's maximum and sum
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float wm = warp_max(m);
+  double ws = (m > -INFINITY && (wm < INFINITY || m == wm)) ? (double)s * (m == wm ? 1.0 : exp((double)m - (double)wm)) : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+  if (lane == 0) {
+    sh.red_m[warp] = wm;
+    sh.red_s[warp] = ws;
+  }
+  const int n = beam_compact(keep, log2_lanes, sh);
+  if (threadIdx.x == 0) {
+    float am = sh.red_m[0];
+    for (int w = 1; w < BEAM_THREADS / 32; ++w) am = fmaxf(am, sh.red_m[w]);
+    double as = 0.0;
+    for (int w = 0; w < BEAM_THREADS / 32; ++w)
+      if (sh.red_m[w] > -INFINITY && (am < INFINITY || sh.red_m[w] == am)) as += sh.red_s[w] * (sh.red_m[w] == am ? 1.0 : exp((double)sh.red_m[w] - (double)am));
+    parts[blockIdx.x] = BeamPart{as, am};
+  }
+  for (int i = threadIdx.x; i < keep; i += BEAM_THREADS) keys[(size_t)blockIdx.x * keep + i] = i < n ? sh.list[i] : 0ull;
+}
+
+// A search: warp b joins the parts of beam b's row, then the first warp joins the beams.  Every step of a join takes the largest of the lists' heads.
+__global__ void beam_merge_kernel(const float* scores, const BeamPart* parts, const unsigned long long* keys, int B, int keep, int splits, float* out_score, int* out_parent,
+                                  int* out_token) {
+  extern __shared__ __align__(16) unsigned char beam_smem[];
+  unsigned long long* lists = reinterpret_cast<unsigned long long*>(beam_smem);        // [B][splits][keep]: a beam's parts
+  unsigned long long* head_score = lists + (size_t)B * splits * keep;                  // [B][keep]: a beam's scores, joined
+  int* best_token = reinterpret_cast<int*>(head_score + B * keep);                     // [B][keep]
+  pdl_launch_dependents();
+  pdl_wait();
+  const int g = blockIdx.x, b = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const size_t row = (size_t)g * B + b;
+  const float score = scores[row];
+  {
+    unsigned long long* mine = lists + (size_t)b * splits * keep;
+    const unsigned long long* src = keys + row * splits * keep;
+    for (int i = lane; i < splits * keep; i += 32) mine[i] = src[i];
+    float top = -INFINITY;
+    for (int p = lane; p < splits; p += 32) top = fmaxf(top, parts[row * splits + p].max);
+    top = warp_max(top);
+    double sum = 0.0;
+    for (int p = lane; p < splits; p += 32) {
+      const BeamPart q = parts[row * splits + p];
+      if (q.max == top) sum += q.sum;
+      else if (top < INFINITY && q.max > -INFINITY) sum += q.sum * exp((double)q.max - (double)top);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double lse = log(sum);
+    const bool alive = score > -INFINITY && top > -INFINITY;
+    __syncwarp();
+    int n = 0;
+    if (alive) {                                    // lane l walks the l-th part's list
+      int at = 0;
+      unsigned long long head = lane < splits ? mine[lane * keep] : 0ull;
+      for (; n < keep; ++n) {
+        const unsigned long long best = warp_max_key(head);
+        if (best == 0) break;
+        if (lane == 0) {
+          const float x = beam_value((uint32_t)(best >> 32));
+          const double d = x == top ? 0.0 : (double)x - (double)top;
+          const double v = (double)score + (d - lse);
+          head_score[b * keep + n] = v > -INFINITY ? order_double(v) : 0ull;
+          best_token[b * keep + n] = (int)~(uint32_t)best;
+        }
+        if (head == best) {
+          ++at;
+          head = at < keep ? mine[lane * keep + at] : 0ull;
+        }
+      }
+    }
+    for (int i = n + lane; i < keep; i += 32) head_score[b * keep + i] = 0;
+  }
+  __syncthreads();
+  if (b != 0) return;
+  int at = 0;
+  unsigned long long head = lane < B ? head_score[lane * keep] : 0ull;
+  for (int n = 0; n < keep; ++n) {
+    const unsigned long long best = warp_max_key(head);
+    const size_t o = (size_t)g * keep + n;
+    if (best == 0) {
+      if (lane == 0) {
+        out_score[o] = -INFINITY;
+        out_parent[o] = -1;
+        out_token[o] = -1;
+      }
+      continue;
+    }
+    const int who = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;       // of equal scores the first beam's
+    if (lane == who) {
+      out_score[o] = (float)double_of(best);
+      out_parent[o] = lane;
+      out_token[o] = best_token[lane * keep + at];
+      ++at;
+      head = at < keep ? head_score[lane * keep + at] : 0ull;
+    }
+  }
+}
+
+// ---- what goes on and what is finished ------------------------------------------------------------------------------------
+//
+// A warp a search.  The candidates come in their order; stop tokens among the first `beams` of them are finished continuations, scored s / n^power with n the tokens
+// so far; the first `beams` that are none go on.  At n = max_new what would go on is finished too.  The pool holds the W best finished ones in order (of equal
+// scores the earlier), lane w the w-th.  The search is over when nothing goes on, at max_new, or when the pool is full and the best that goes on cannot
+// get above its last: log-probabilities only fall, so it ends at best at best / max_new^power (power >= 0) or best / (n + 1)^power (power < 0).
+struct BeamPool {
+  float* score;
+  int *length, *parent, *token;
+};
+
+__device__ __forceinline__ float beam_norm(float s, int n, double power) { return (float)((double)s / pow((double)n, power)); }
+
+__global__ void __launch_bounds__(32) beam_advance_kernel(const float* c_score, const int* c_parent, const int* c_token, int keep, int beams, int W, const float* p_score,
+                                                          const int* p_length, const int* p_parent, const int* p_token, const int* lengths, const int* done, const int* stop_ids,
+                                                          int stops, int max_new, double power, float* out_score, int* out_parent, int* out_token, BeamPool pool,
+                                                          int* out_lengths, int* out_done) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int g = blockIdx.x, lane = threadIdx.x;
+  const unsigned full = 0xffffffffu;
+  float ps = -INFINITY;
+  int pl = 0, pp = 0, pt = 0;
+  if (lane < W) {
+    ps = p_score[(size_t)g * W + lane];
+    if (ps > -INFINITY) {
+      pl = p_length[(size_t)g * W + lane];
+      pp = p_parent[(size_t)g * W + lane];
+      pt = p_token[(size_t)g * W + lane];
+    } else {
+      ps = -INFINITY;
+    }
+  }
+  const bool was_done = done[g] != 0;
+  const int before = lengths[g], n = before + 1;
+  bool over = was_done;
+  constexpr int PER = BEAM_KEEP / 32;
+  float cs[PER];
+  int cp[PER], ct[PER], place[PER];              // place: among those that go on, -1: not one of them
+  int live = 0;
+  float lead = -INFINITY;
+  if (!was_done) {
+    unsigned stop_mask[PER];
+    auto enter = [&](float s, int parent, int token) {        // uniform
+      const float v = beam_norm(s, n, power);
+      const int at = __popc(__ballot_sync(full, lane < W && ps >= v));
+      const float us = __shfl_up_sync(full, ps, 1);
+      const int ul = __shfl_up_sync(full, pl, 1), up = __shfl_up_sync(full, pp, 1), ut = __shfl_up_sync(full, pt, 1);
+      if (lane < W && lane >= at && v > -INFINITY) {
+        ps = lane == at ? v : us;
+        pl = lane == at ? n : ul;
+        pp = lane == at ? parent : up;
+        pt = lane == at ? token : ut;
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int r = 32 * j + lane;
+      const bool in = r < keep;
+      cs[j] = in ? c_score[(size_t)g * keep + r] : -INFINITY;
+      cp[j] = in ? c_parent[(size_t)g * keep + r] : -1;
+      ct[j] = in ? c_token[(size_t)g * keep + r] : -1;
+      bool stop = false;
+      for (int k = 0; k < stops; ++k) stop |= stop_ids[k] == ct[j];
+      const bool there = cs[j] > -INFINITY;
+      stop_mask[j] = __ballot_sync(full, there && stop && r < beams);
+      const unsigned goes = __ballot_sync(full, there && !stop);
+      const int mine = live + __popc(goes & ((1u << lane) - 1));
+      place[j] = (there && !stop && mine < beams) ? mine : -1;
+      const unsigned first = __ballot_sync(full, place[j] == 0);
+      if (first) lead = __shfl_sync(full, cs[j], __ffs(first) - 1);
+      live += __popc(goes);
+    }
+    live = live < beams ? live : beams;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      for (unsigned mask = stop_mask[j]; mask; mask &= mask - 1) {
+        const int l = __ffs(mask) - 1;
+        enter(__shfl_sync(full, cs[j], l), __shfl_sync(full, cp[j], l), __shfl_sync(full, ct[j], l));
+      }
+    if (n >= max_new) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        for (unsigned mask = __ballot_sync(full, place[j] >= 0); mask; mask &= mask - 1) {
+          const int l = __ffs(mask) - 1;
+          enter(__shfl_sync(full, cs[j], l), __shfl_sync(full, cp[j], l), __shfl_sync(full, ct[j], l));
+        }
+      over = true;
+    }
+    const float last = __shfl_sync(full, ps, W - 1);
+    if (live == 0) over = true;
+    else if (last > -INFINITY && beam_norm(lead, power >= 0.0 ? max_new : n + 1, power) <= last) over = true;
+  }
+  // the next beams: those that go on, in order; the others of them idle (parent -1), or all of them where the search is over
+  if (lane < beams && (over || lane >= live)) {
+    out_score[(size_t)g * beams + lane] = -INFINITY;
+    out_parent[(size_t)g * beams + lane] = over ? lane : -1;
+    out_token[(size_t)g * beams + lane] = 0;
+  }
+  if (!over) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (place[j] >= 0) {
+        out_score[(size_t)g * beams + place[j]] = cs[j];
+        out_parent[(size_t)g * beams + place[j]] = cp[j];
+        out_token[(size_t)g * beams + place[j]] = ct[j];
+      }
+  }
+  if (lane < W) {
+    pool.score[(size_t)g * W + lane] = ps;
+    pool.length[(size_t)g * W + lane] = pl;
+    pool.parent[(size_t)g * W + lane] = pp;
+    pool.token[(size_t)g * W + lane] = pt;
+  }
+  if (lane == 0) {
+    out_lengths[g] = was_done ? before : n;
+    out_done[g] = over ? 1 : 0;
+  }
+}
+
+static size_t beam_merge_smem(int B, int splits, int keep) { return (size_t)B * keep * (8 * splits + 12); }
+
+static int beam_log2_lanes(int keep) {             // four groups a wanted key, where the threads suffice
+  int lg = 5;
+  while (lg > 0 && (BEAM_THREADS >> lg) < 4 * keep) --lg;
+  return lg;
+}
+
+}  // namespace sllm
+
+using namespace sllm;
+
+// parts a row is cut into, at most 32 (a lane of the merging warp each)
+SLLM_EXPORT int sllm_beam_splits(int G, int B, int V, int keep) { return 1; }
+
+// scratch: G * B * splits * (8 * keep + 16) bytes, every part's keys, then its sum and maximum
+SLLM_EXPORT int sllm_beam_candidates(const void* logits, int dtype, const float* scores, int G, int B, int V, int keep, int splits, void* scratch, float* out_score, int* out_parent,
+                                     int* out_token, cudaStream_t stream) {
+  SLLM_REQUIRE(G >= 0 && B >= 1 && B <= BEAM_MAX && V >= 1 && keep >= 1 && keep <= BEAM_KEEP && (long long)G * B < (1ll << 24), "beam_candidates: %d searches of %d beams, %d logits, %d kept", G, B, V,
+               keep);
+  SLLM_REQUIRE(V <= (1 << 30), "beam_candidates: rows of %d logits", V);
+  SLLM_REQUIRE(dtype == SLLM_F32 || dtype == SLLM_BF16, "beam_candidates: unknown dtype %d", dtype);
+  SLLM_REQUIRE(splits >= 1 && splits <= 32 && (long long)G * B * splits < (1ll << 31), "beam_candidates: %d parts a row", splits);
+  if (G == 0) return SLLM_OK;
+  const int lanes = beam_log2_lanes(keep);
+  const int per = dtype == SLLM_F32 ? 4 : 8;
+  const int part_vecs = ((V + per - 1) / per + splits - 1) / splits;
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(scratch);
+  BeamPart* parts = reinterpret_cast<BeamPart*>(keys + (size_t)G * B * splits * keep);
+  static SharedLimit limit_f, limit_b, limit_m;
+  const size_t merge_smem = beam_merge_smem(B, splits, keep);
+  if (!(dtype == SLLM_F32 ? limit_f.raise(beam_rows_kernel<float>, sizeof(BeamShared)) : limit_b.raise(beam_rows_kernel<__nv_bfloat16>, sizeof(BeamShared))) ||
+      !limit_m.raise(beam_merge_kernel, merge_smem)) {
+    set_error("beam_candidates: cannot raise the shared memory limit");
+    return SLLM_ERR_LAUNCH;
+  }
+  if (dtype == SLLM_F32)
+    launch_kernel(beam_rows_kernel<float>, dim3((unsigned)(G * B * splits)), BEAM_THREADS, sizeof(BeamShared), stream, (const float*)logits, V, keep, lanes, splits, part_vecs, parts, keys);
+  else
+    launch_kernel(beam_rows_kernel<__nv_bfloat16>, dim3((unsigned)(G * B * splits)), BEAM_THREADS, sizeof(BeamShared), stream, (const __nv_bfloat16*)logits, V, keep, lanes, splits, part_vecs, parts,
+                  keys);
+  launch_kernel(beam_merge_kernel, G, 32 * B, merge_smem, stream, scores, (const BeamPart*)parts, (const unsigned long long*)keys, B, keep, splits, out_score, out_parent, out_token);
+  return launch_status("beam_candidates");
+}
+
+// `power` (on the host): the length penalty.  What is read may be what is written.
+SLLM_EXPORT int sllm_beam_advance(const float* c_score, const int* c_parent, const int* c_token, int G, int keep, int beams, int W, const float* p_score, const int* p_length,
+                                  const int* p_parent, const int* p_token, const int* lengths, const int* done, const int* stop_ids, int stops, int max_new, const double* power,
+                                  float* out_score, int* out_parent, int* out_token, float* out_p_score, int* out_p_length, int* out_p_parent, int* out_p_token, int* out_lengths,
+                                  int* out_done, cudaStream_t stream) {
+  SLLM_REQUIRE(G >= 0 && keep >= 1 && keep <= BEAM_KEEP && beams >= 1 && beams <= BEAM_MAX && W >= 1 && W <= 32 && stops >= 0 && max_new >= 1,
+               "beam_advance: %d searches, %d candidates, %d beams, a pool of %d, %d stops, max_new %d", G, keep, beams, W, stops, max_new);
+  if (G == 0) return SLLM_OK;
+  launch_kernel(beam_advance_kernel, G, 32, 0, stream, c_score, c_parent, c_token, keep, beams, W, p_score, p_length, p_parent, p_token, lengths, done, stop_ids, stops, max_new, *power,
+                out_score, out_parent, out_token, BeamPool{out_p_score, out_p_length, out_p_parent, out_p_token}, out_lengths, out_done);
+  return launch_status("beam_advance");
+}

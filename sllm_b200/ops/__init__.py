@@ -2617,3 +2617,235 @@ def penalty_from_seen_(logits: torch.Tensor, seen: torch.Tensor, step, penalty: 
     call("sllm_penalty_seen", _p(logits), R, V, _p(seen), seen.shape[0], _p(step.logit_rows), _p(step.seq_of_token),
          _p(step.state_slots), _p(penalty), _stream())
     return logits
+
+
+# ---- beam search ------------------------------------------------------------------------------------------------------
+
+MAX_BEAMS, MAX_CANDIDATES, MAX_BEAM_ROWS = 32, 128, 2048
+
+BeamPool = namedtuple("BeamPool", "scores lengths parents tokens")
+BeamStep = namedtuple("BeamStep", "scores parents tokens lengths done pool")
+StepTables = namedtuple("StepTables", "q_start ctx_len positions seq_of_token block_tables slot_mappings")
+
+
+def _one_device(what: str, *tensors) -> None:
+    """All on the current device: the launch goes to its current stream."""
+    index = _current_device() if _current_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != index:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{index}")
+
+
+def _typed(what: str, dtype, shape, *tensors) -> None:
+    for t in tensors:
+        if t.dtype != dtype or tuple(t.shape) != shape:
+            raise KernelError(f"{what}: {t.dtype} {tuple(t.shape)}, not {dtype} {shape}")
+
+
+def beam_candidates(logits: torch.Tensor, scores: torch.Tensor, keep: int):
+    """The best continuations of ``G`` searches of ``B`` beams: ``logits`` (float32 or bfloat16 ``[G*B, V]``) of the beams' next
+    tokens, ``scores`` (float32 ``[G, B]``) their cumulative log-probabilities.  Of all beams and tokens of a search the ``keep`` largest
+    ``score + log_softmax(logits)``, in order: by that sum (compared in 64 bits), then the lower beam, the larger logit, the lower token.
+    Returns ``(scores float32, beams int32, tokens int32)``, each ``[G, keep]``.
+
+    A beam whose score is minus infinity or not a number takes no part, nor does a logit that is; where there are fewer
+    candidates the rest is minus infinity, beam -1, token -1.  At most 32 beams and 128 candidates a search."""
+    _chk(logits, scores)
+    _one_device("beam_candidates", logits, scores)
+    if logits.dim() != 2 or scores.dim() != 2 or scores.dtype != torch.float32 or logits.shape[0] != scores.numel():
+        raise KernelError(f"beam_candidates: logits {tuple(logits.shape)} and {scores.dtype} scores {tuple(scores.shape)}, not [G*B, V] and float32 [G, B]")
+    (G, B), V, keep, dt = scores.shape, logits.shape[1], int(keep), _dt(logits)
+    if not 1 <= B <= MAX_BEAMS or not 1 <= keep <= MAX_CANDIDATES or V < 1:
+        raise KernelError(f"beam_candidates: {B} beams (1 to {MAX_BEAMS}), {keep} candidates (1 to {MAX_CANDIDATES}), {V} logits")
+    dev = logits.device
+    out_s = torch.empty((G, keep), dtype=torch.float32, device=dev)
+    out_i = torch.empty((2, G, keep), dtype=torch.int32, device=dev)
+    parents, tokens = out_i.unbind(0)
+    if G == 0:
+        return out_s, parents, tokens
+    splits = lib().sllm_beam_splits(G, B, V, keep)
+    scratch = torch.empty(G * B * splits * (keep + 2), dtype=torch.int64, device=dev)
+    call("sllm_beam_candidates", _p(logits), dt, _p(scores), G, B, V, keep, splits, _p(scratch), _p(out_s), _p(parents), _p(tokens), _stream())
+    return out_s, parents, tokens
+
+
+def beam_pool(searches: int, width: int, device) -> BeamPool:
+    """An empty pool of finished continuations for `beam_advance`: the ``width`` best of each search."""
+    return BeamPool(torch.full((searches, width), -float("inf"), dtype=torch.float32, device=device),
+                    *(torch.zeros((searches, width), dtype=torch.int32, device=device) for _ in range(3)))
+
+
+def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beams: int, stop_ids=None, max_new: int,
+                 length_penalty: float = 1.0, out: "BeamStep | None" = None) -> BeamStep:
+    """What of the candidates (``[G, keep]`` each, as `beam_candidates` gives them) goes on and what is finished.
+
+    ``lengths`` (int32 ``[G]``) tokens have been generated before; the candidates' are the n-th, n = lengths + 1.  A candidate whose token
+    is one of ``stop_ids`` (int32 ``[n]``) and that stands among the first ``beams`` is finished; the first ``beams`` that are no stops go
+    on (at n = ``max_new`` they are finished too, behind the stops).  What is finished enters ``pool`` (a `BeamPool` ``[G, W]``, best first; of equal scores the
+    earlier stays in front) with score ``s / n ** length_penalty``, length n, its beam before the token, and the token; an empty
+    place is minus infinity and zeros.  A search is over (``done`` int32 ``[G]``) once nothing goes on, n reaches ``max_new``, or its pool is full and
+    no log-probability could lift the best that goes on above the pool's last: going on would not change the pool.
+
+    Returns a `BeamStep`: ``scores``, ``parents`` and ``tokens`` ``[G, beams]`` of the next beams (fewer than ``beams``: minus infinity, -1,
+    0; a search that is over: minus infinity, each beam its own parent, 0), the new ``lengths``, ``done`` and ``pool``; a search that was over before keeps
+    its pool and length.  ``out``: a `BeamStep` of tensors to write, the inputs' own among them.  At most 32 beams, a pool of 32 and 128 candidates."""
+    if out is None:
+        out = BeamStep(*(None,) * 5, BeamPool(*(None,) * 4))
+    given = (scores, parents, tokens, *pool, lengths, done)
+    _chk(*given, stop_ids, *out[:5], *out.pool)
+    _one_device("beam_advance", *given, stop_ids, *out[:5], *out.pool)
+    if scores.dim() != 2 or pool.scores.dim() != 2:
+        raise KernelError("beam_advance: candidates [G, keep] and a pool [G, W]")
+    (G, keep), W, beams, max_new, power = scores.shape, pool.scores.shape[1], int(beams), int(max_new), float(length_penalty)
+    if not 1 <= keep <= MAX_CANDIDATES or not 1 <= beams <= MAX_BEAMS or not 1 <= W <= MAX_BEAMS or not 1 <= max_new < 1 << 30 or not abs(power) < 64:
+        raise KernelError(f"beam_advance: {keep} candidates (1 to {MAX_CANDIDATES}), {beams} beams and a pool of {W} (1 to {MAX_BEAMS}), "
+                          f"max_new {max_new}, length penalty {power}")
+    _typed("beam_advance: scores", torch.float32, (G, keep), scores)
+    _typed("beam_advance: parents and tokens", torch.int32, (G, keep), parents, tokens)
+    _typed("beam_advance: the pool's scores", torch.float32, (G, W), pool.scores)
+    _typed("beam_advance: the pool's lengths, parents and tokens", torch.int32, (G, W), *pool[1:])
+    _typed("beam_advance: lengths and done", torch.int32, (G,), lengths, done)
+    if stop_ids is not None and stop_ids.dtype != torch.int32:
+        raise KernelError("beam_advance: stop ids are int32")
+    dev = scores.device
+    shapes = BeamStep(*(((G, beams), torch.float32),), *((((G, beams), torch.int32),) * 2), *((((G,), torch.int32),) * 2),
+                      (((G, W), torch.float32),) + (((G, W), torch.int32),) * 3)
+
+    def place(t, what):
+        if t is None:
+            return torch.empty(what[0], dtype=what[1], device=dev)
+        _typed("beam_advance: out", what[1], what[0], t)
+        return t
+    res = BeamStep(*(place(t, w) for t, w in zip(out[:5], shapes[:5])), BeamPool(*(place(t, w) for t, w in zip(out.pool, shapes.pool))))
+    if G:
+        call("sllm_beam_advance", _p(scores), _p(parents), _p(tokens), G, keep, beams, W, *(_p(t) for t in pool), _p(lengths), _p(done),
+             _p(stop_ids), stop_ids.numel() if stop_ids is not None else 0, max_new, ctypes.byref(ctypes.c_double(power)),
+             _p(res.scores), _p(res.parents), _p(res.tokens), *(_p(t) for t in res.pool), _p(res.lengths), _p(res.done), _stream())
+    return res
+
+
+def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
+    """States and pages follow the beams: beam i of each search goes on from what beam ``parents[i]`` (int32 ``[G, B]``) holds.
+
+    ``slots`` (int32 ``[G*B]``) names each beam's row in every tensor of ``states`` (``[rows, ...]``, any type); ``paged`` lists
+    ``(storage [..., pages, heads, page size, head size], block table int32 [G*B, columns], stride)``, caches that hold an entry per ``stride`` tokens; ``lens``
+    (int32 ``[G]``) tokens are in a search's caches.  A parent's first child keeps its slot and its page that is only partly written; the other children get copies
+    of the row and of the page's entries, in the slots and pages of beams without a child, in order; pages before that one are shared, those behind it stay each
+    beam's own.  A beam with parent -1 takes such a place as it is.  Each slot, and each page from the first that is partly written on, belongs to one beam.
+
+    Returns ``(new slots, [new block tables])``; ``out`` is such a pair of tensors to write (others than those read).  At most 32 beams a search, 2,048 in all."""
+    states, paged = list(states), [(s, t, int(st)) for s, t, st in paged]
+    new_slots, tables = out if out is not None else (None, [None] * len(paged))
+    _chk(parents, slots, lens, *states, *(x for p in paged for x in p[:2]), new_slots, *tables)
+    _one_device("beam_reorder", parents, slots, lens, *states, *(x for p in paged for x in p[:2]), new_slots, *tables)
+    if parents.dim() != 2 or len(tables) != len(paged):
+        raise KernelError(f"beam_reorder: parents {tuple(parents.shape)}, not [G, B], or {len(tables)} tables for {len(paged)} caches")
+    G, B = parents.shape
+    if not 1 <= B <= MAX_BEAMS or G * B > MAX_BEAM_ROWS:
+        raise KernelError(f"beam_reorder: {G} searches of {B} beams (at most {MAX_BEAMS}, {MAX_BEAM_ROWS} in all)")
+    _typed("beam_reorder: parents", torch.int32, (G, B), parents)
+    _typed("beam_reorder: slots", torch.int32, (G * B,), slots)
+    _typed("beam_reorder: lens", torch.int32, (G,), lens)
+    if new_slots is None:
+        new_slots = torch.empty_like(slots)
+    _typed("beam_reorder: new slots", torch.int32, (G * B,), new_slots)
+    about, made, read = [], [], {slots.data_ptr()}
+    for (storage, table, stride), new in zip(paged, tables):
+        if storage.dim() < 4 or stride < 1 or storage.element_size() < 2:
+            raise KernelError(f"beam_reorder: a cache {storage.dtype} {tuple(storage.shape)}, an entry per {stride} tokens")
+        if table.dim() != 2:
+            raise KernelError("beam_reorder: a block table has a row a beam")
+        _typed("beam_reorder: a block table", torch.int32, (G * B, table.shape[1]), table)
+        if new is None:
+            new = torch.empty_like(table)
+        _typed("beam_reorder: a new block table", torch.int32, tuple(table.shape), new)
+        made.append(new)
+        read.add(table.data_ptr())
+        pages, heads, page_size, dim = storage.shape[-4:]
+        if storage.numel() == 0:
+            raise KernelError("beam_reorder: a cache without pages")
+        if table.numel():
+            outer = storage.numel() // (pages * heads * page_size * dim)
+            about += (storage.data_ptr(), table.data_ptr(), new.data_ptr(), dim * storage.element_size(), outer, heads, pages, page_size, stride, table.shape[1])
+    if G == 0:
+        return new_slots, made
+    if any(t.numel() and t.data_ptr() in read for t in (new_slots, *made)):
+        raise KernelError("beam_reorder: what is written cannot be what is read")
+    rows = []
+    for t in states:
+        if t.dim() < 1:
+            raise KernelError("beam_reorder: a state has a row a slot")
+        if t.numel():
+            rows += (t.data_ptr(), t.numel() // t.shape[0] * t.element_size(), t.shape[0])
+    first = True
+    while first or rows or about:             # (64 states and 8 caches a launch)
+        s, p = rows[:3 * 64], about[:10 * 8]
+        rows, about = rows[3 * 64:], about[10 * 8:]
+        call("sllm_beam_reorder", _p(parents), _p(slots), _p(lens), _p(new_slots) if first else None, G, B, (ctypes.c_longlong * len(s))(*s), len(s) // 3,
+             (ctypes.c_longlong * len(p))(*p), len(p) // 10, _stream())
+        first = False
+    return new_slots, made
+
+
+def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, strides=None, rows=None, free=None, columns=None,
+                out: "StepTables | None" = None) -> StepTables:
+    """A step's description from the requests' lengths: request s brings ``q_lens[s]`` tokens behind the ``have[s]`` it holds (int32
+    ``[S]``), ``num_tokens`` in all.  ``page_tables`` gives, per cache group, the pages of every live request in order (int32 ``[N, columns]``); request s has row
+    ``rows[s]`` (int32 ``[S]``, each row once; None: row s).  A group holds one entry per ``strides[k]`` tokens (None: per token), ``page_size`` entries a page.
+
+    Returns a `StepTables` of int32 tensors: ``q_start [S+1]``, ``ctx_len [S]``, ``positions [T]`` and ``seq_of_token [T]``, and per group ``block_tables [S, columns]``
+    (``columns[k]`` of them; None: as many as the page table has), the request's pages up to its new length and -1 behind, and ``slot_mappings [T]``, the entry that a token
+    writes: page times ``page_size`` plus place, or -1 (a token that completes no block of ``stride``; a page that the table does not have).  With more ``num_tokens`` than the
+    requests bring, the rows behind them have position 0, request 0 and slot -1; with fewer, tokens are left out.
+
+    ``free`` (int32 ``[n]`` per group): pages that nobody holds.  A request whose new tokens need further pages takes them from there, in the order of the requests, and they
+    are written into its row of the page table; where the list is too short, -1.  ``out``: a `StepTables` of tensors to write."""
+    page_tables = list(page_tables)
+    n, T, page_size = len(page_tables), int(num_tokens), int(page_size)
+    strides = [1] * n if strides is None else [int(s) for s in strides]
+    free = [None] * n if free is None else list(free)
+    columns = [None] * n if columns is None else list(columns)
+    if len(strides) != n or len(free) != n or len(columns) != n or n > 8:
+        raise KernelError(f"step_tables: {n} groups (8 at most), {len(strides)} strides, {len(free)} lists of free pages, {len(columns)} numbers of columns")
+    flat = (q_lens, have, rows, *page_tables, *free) + ((*out[:4], *out.block_tables, *out.slot_mappings) if out is not None else ())
+    _chk(*flat)
+    _one_device("step_tables", *flat)
+    S = q_lens.numel()
+    if S < 1 or T < 0 or page_size < 1 or any(s < 1 for s in strides):
+        raise KernelError(f"step_tables: {S} requests, {T} tokens, pages of {page_size}, strides {strides}")
+    _typed("step_tables: lengths", torch.int32, (S,), q_lens, have)
+    if rows is not None:
+        _typed("step_tables: rows", torch.int32, (S,), rows)
+    N = page_tables[0].shape[0] if n else S
+    for t, f in zip(page_tables, free):
+        if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] != N or N < 1 or (rows is None and N < S):
+            raise KernelError(f"step_tables: a page table {t.dtype} {tuple(t.shape)}, not int32 [{N}, columns] with a row for each of {S} requests")
+        if f is not None and (f.dtype != torch.int32 or f.dim() != 1):
+            raise KernelError("step_tables: free pages are an int32 list")
+    columns = [t.shape[1] if c is None else int(c) for t, c in zip(page_tables, columns)]
+    if any(c < 0 for c in columns):
+        raise KernelError(f"step_tables: {columns} columns")
+    if out is None:
+        dev = q_lens.device
+        per_seq = torch.empty(2 * S + 1, dtype=torch.int32, device=dev)
+        per_token = torch.empty((2 + n, T), dtype=torch.int32, device=dev).unbind(0)
+        out = StepTables(per_seq[:S + 1], per_seq[S + 1:], per_token[0], per_token[1],
+                         tuple(torch.empty((S, c), dtype=torch.int32, device=dev) for c in columns), tuple(per_token[2:]))
+    else:
+        _typed("step_tables: out.q_start", torch.int32, (S + 1,), out.q_start)
+        _typed("step_tables: out.ctx_len", torch.int32, (S,), out.ctx_len)
+        _typed("step_tables: out, per token", torch.int32, (T,), out.positions, out.seq_of_token, *out.slot_mappings)
+        if len(out.block_tables) != n or len(out.slot_mappings) != n:
+            raise KernelError("step_tables: out has other groups")
+        for t, c in zip(out.block_tables, columns):
+            _typed("step_tables: out.block_tables", torch.int32, (S, c), t)
+        read = {t.data_ptr() for t in (q_lens, have, *page_tables) if t.numel()}
+        if any(t.numel() and t.data_ptr() in read for t in (*out[:4], *out.block_tables, *out.slot_mappings)):
+            raise KernelError("step_tables: what is written cannot be what is read")
+    about = []
+    for t, f, c, st, b, m in zip(page_tables, free, columns, strides, out.block_tables, out.slot_mappings):
+        # (an empty list of free pages is still a list: its pointer only has to be one)
+        about += (t.data_ptr(), 0 if f is None else (f.data_ptr() or t.data_ptr()), b.data_ptr(), m.data_ptr(), t.shape[1], c, 0 if f is None else f.numel(), st)
+    call("sllm_step_tables", _p(q_lens), _p(have), _p(rows), S, N, T, page_size, _p(out.q_start), _p(out.ctx_len), _p(out.positions), _p(out.seq_of_token),
+         (ctypes.c_longlong * len(about))(*about), n, _stream())
+    return out

@@ -1,0 +1,342 @@
+"""The operators of a beam search against their definitions in float64 (tests/plain/beam_plain.py).  Whole numbers are equal; scores are float32 roundings of a float64 sum whose
+only float32 part are the exponentials, see `SCORE`."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests.conftest import cuda_or_skip
+from tests.plain import beam_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+# A score s + (d - log sum) off by: the rounding of the result (2^-24 of it), and the relative error of the sum of exponentials, which an exponential of a rounded difference
+# |d| <= 32 can have (2^-24 * 32 for the difference, 2 units for expf, 2^-24 * 40 for a thread's up to 600 terms in pairs of partial sums).
+SCORE = lambda s: 2.0 ** -24 * np.abs(s) + 2.0 ** -24 * (32 + 2 + 40)      # noqa: E731
+
+
+def _i32(a, dev):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device=dev)
+
+
+def _check_candidates(logits, scores, keep, gap=2e-6):
+    """Every place of every search.  Where two candidates of different beams lie closer than the scores' own error the order is not tested (the inputs keep away from that but for
+    equal rows, which are equal in every bit)."""
+    import sllm_b200.ops as ops
+    s, p, t = (x.cpu().numpy() for x in ops.beam_candidates(logits, scores, keep))
+    G, B = scores.shape
+    rows = logits.float().cpu().numpy().reshape(G, B, -1)
+    for g in range(G):
+        want = plain.candidates(rows[g], scores[g].cpu().numpy(), keep)
+        n = len(want)
+        assert (s[g, n:] == -np.inf).all() and (p[g, n:] == -1).all() and (t[g, n:] == -1).all()
+        if not n:
+            continue
+        ws, wb, wt = (np.array(x) for x in zip(*want))
+        assert (np.abs(s[g, :n] - ws) <= SCORE(ws)).all() or np.array_equal(s[g, :n], ws.astype(np.float32)), (g, np.abs(s[g, :n] - ws).max())
+        assert np.array_equal(p[g, :n], wb) and np.array_equal(t[g, :n], wt), (g, np.flatnonzero((p[g, :n] != wb) | (t[g, :n] != wt))[:5])
+
+
+@pytest.mark.parametrize("V", [1, 3, 260, 1021, 4096, 32001, 151936])
+@pytest.mark.parametrize("G,B,keep", [(1, 1, 1), (1, 4, 8), (3, 5, 15), (2, 32, 128), (9, 2, 33)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_candidates(V, G, B, keep, dtype):
+    dev = cuda_or_skip()
+    g = torch.Generator(device=dev).manual_seed(V + 7 * G + B)
+    logits = (torch.randn(G * B, V, device=dev, generator=g) * 3).to(dtype)
+    scores = -torch.rand(G, B, device=dev, generator=g) * 5
+    _check_candidates(logits, scores, keep)
+
+
+@pytest.mark.parametrize("V", [40, 5003, 33000])
+@pytest.mark.parametrize("keep", [1, 6, 40, 128])
+def test_candidates_of_odd_rows(V, keep):
+    """Dead beams, masked tokens, rows with nothing, not a number, infinities, ties, sorted rows, equal rows, both zeros."""
+    dev = cuda_or_skip()
+    g = torch.Generator(device=dev).manual_seed(V + keep)
+    G, B = 5, 6
+    x = torch.randn(G, B, V, device=dev, generator=g) * 2
+    scores = -torch.rand(G, B, device=dev, generator=g) * 5
+    scores[0, 1], scores[0, 2] = -math.inf, math.nan
+    x[0, 3] = -math.inf
+    x[0, 4, ::3] = math.nan
+    x[0, 5, : V - 2] = -math.inf
+    x[1] = x[1].round()                                        # ties within a row
+    x[2, 0] = x[2, 0].sort().values                            # every logit above the ones before
+    x[2, 1] = x[2, 1].sort(descending=True).values
+    x[2, 2] = 0.0                                              # all equal
+    x[2, 3] = torch.finfo(torch.float32).min                   # the type's lowest value everywhere: equal too
+    x[2, 4, 1:] = torch.finfo(torch.float32).min               # and behind one that counts
+    x[2, 5, 7:9], x[2, 5, 9:11] = -0.0, 0.0
+    x[3] = x[3, 0]                                             # equal rows and equal scores: the lower beam first
+    scores[3] = scores[3, 0]
+    x[4, 0, 5], x[4, 0, V - 1] = math.inf, math.inf            # an infinite maximum takes all
+    x[4, 1] = -math.inf
+    scores[4, 2:] = -math.inf
+    _check_candidates(x.reshape(G * B, V).contiguous(), scores, keep)
+
+
+def test_candidates_of_rows_off_their_alignment():
+    """Rows that begin on any element, a storage that does too."""
+    dev = cuda_or_skip()
+    for dtype in (torch.float32, torch.bfloat16):
+        for V in (5, 1003, 8191):
+            for off in (1, 2, 3):
+                flat = torch.randn(6 * V + off, device=dev, generator=torch.Generator(device=dev).manual_seed(V + off)).to(dtype)
+                _check_candidates(flat[off:].view(6, V), -torch.rand(2, 3, device=dev), 7)
+
+
+def test_candidates_far_apart_scores_and_large_logits():
+    dev = cuda_or_skip()
+    g = torch.Generator(device=dev).manual_seed(5)
+    x = torch.randn(8, 3001, device=dev, generator=g) * 40 + 500
+    scores = torch.tensor([[-3.0, -900.0, -3.5, -40.0], [0.0, -1e-3, -2.0, -5000.0]], device=dev)
+    _check_candidates(x, scores, 24)
+
+
+def test_candidates_of_no_search():
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    s, p, t = ops.beam_candidates(torch.empty(0, 50, device=dev), torch.empty(0, 4, device=dev), 8)
+    assert s.shape == p.shape == t.shape == (0, 8)
+
+
+def _random_step(rng, G, B, K, stops, full):
+    stop = list(range(1, 1 + stops))
+    s = -np.sort(rng.uniform(1, 9, (G, K)).astype(np.float32).round(2), axis=1)          # (ties among them)
+    p, t = rng.integers(0, B, (G, K)), rng.integers(5, 50, (G, K))
+    if stops:
+        at = rng.random((G, K)) < 0.4
+        t[at] = rng.choice(stop, at.sum())
+    short = rng.random(G) < 0.3
+    for g in np.flatnonzero(short):
+        n = rng.integers(0, K + 1)
+        s[g, n:], p[g, n:], t[g, n:] = -np.inf, -1, -1
+    W = int(rng.integers(1, 33)) if B > 1 else 1
+    pool = []
+    for g in range(G):
+        n = W if full else int(rng.integers(0, W + 1))
+        held = -np.sort(rng.uniform(0.1, 3, n).astype(np.float32).round(2))
+        pool.append([(v, int(rng.integers(1, 9)), int(rng.integers(0, B)), int(rng.integers(1, 50))) for v in held])
+    return s, p, t, stop, W, pool, rng.integers(0, 12, G), (rng.random(G) < 0.15).astype(int)
+
+
+@pytest.mark.parametrize("B,K", [(1, 1), (1, 3), (4, 8), (7, 40), (32, 128), (20, 5)])
+@pytest.mark.parametrize("stops", [0, 1, 3])
+@pytest.mark.parametrize("power", [0.0, 1.0, 0.7, -0.5])
+def test_advance(B, K, stops, power):
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    for full in (False, True):
+        rng = np.random.default_rng(B * 100 + K + stops)
+        G, max_new = 33, 11
+        s, p, t, stop, W, pool, lengths, done = _random_step(rng, G, B, K, stops, full)
+        flat = [np.array([[e[i] for e in r] + [[-np.inf, 3, 3, 3][i]] * (W - len(r)) for r in pool]) for i in range(4)]
+        held = ops.BeamPool(torch.tensor(flat[0], dtype=torch.float32, device=dev), *(_i32(f, dev) for f in flat[1:]))
+        args = (torch.tensor(s, device=dev), _i32(p, dev), _i32(t, dev))
+        kw = dict(beams=B, stop_ids=_i32(stop, dev) if stops else None, max_new=max_new, length_penalty=power)
+        got = ops.beam_advance(*args, held, _i32(lengths, dev), _i32(done, dev), **kw)
+        # the same into the inputs' own tensors
+        n2, d2 = _i32(lengths, dev), _i32(done, dev)
+        own = ops.BeamPool(*(x.clone() for x in held))
+        again = ops.beam_advance(*args, own, n2, d2, out=ops.BeamStep(None, None, None, n2, d2, own), **kw)
+        assert again.pool.scores.data_ptr() == own.scores.data_ptr() and again.done.data_ptr() == d2.data_ptr()
+        for a, b in zip((*got[:5], *got.pool), (*again[:5], *again.pool)):
+            assert torch.equal(a, b)
+        for g in range(G):
+            nxt, after, n, over = plain.advance(list(zip(s[g], p[g].tolist(), t[g].tolist())), pool[g], int(lengths[g]), int(done[g]), beams=B, stop_ids=stop,
+                                                max_new=max_new, power=power, width=W, seen=got.pool.scores[g].cpu().numpy())
+            after = after + [(-np.inf, 0, 0, 0)] * (W - len(after))
+            for i, x in enumerate(got[:3]):
+                assert x[g].tolist() == [float(e[i]) if i == 0 else e[i] for e in nxt], (g, i)
+            assert (int(got.lengths[g]), int(got.done[g])) == (n, over)
+            assert got.pool.scores[g].tolist() == [float(e[0]) for e in after]
+            for i in (1, 2, 3):
+                assert got.pool[i][g].tolist() == [e[i] for e in after]
+
+
+def _reorder_case(rng, G, B, lens, stride_of, kinds, dev):
+    """Pages of every search: shared whole ones, then one a beam and column; states of several types."""
+    paged = []
+    for (outer, heads, ps, hd, dtype), stride in zip(kinds, stride_of):
+        entries = np.asarray(lens) // stride
+        shared = entries // ps
+        columns = int(shared.max()) + 3
+        pages = int(shared.sum() + G * B * 3 + 4)
+        ids = list(rng.permutation(pages))
+        table = np.full((G * B, columns), -1)
+        for g in range(G):
+            common = [ids.pop() for _ in range(shared[g])]
+            for b in range(B):
+                table[g * B + b, :shared[g]] = common
+                table[g * B + b, shared[g]:shared[g] + 3] = [ids.pop() for _ in range(3)]
+        storage = torch.tensor(rng.integers(-120, 120, outer + (pages, heads, ps, hd)), device=dev).to(dtype)
+        paged.append((storage, table, stride))
+    return paged
+
+
+@pytest.mark.parametrize("G,B", [(1, 1), (1, 2), (3, 4), (5, 7), (2, 32), (64, 32)])
+@pytest.mark.parametrize("dup", [0.0, 0.5, 1.0])
+def test_reorder(G, B, dup):
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    rng = np.random.default_rng(G * 100 + B + int(10 * dup))
+    many = G * B > 500
+    lens = rng.integers(0, 40 if many else 200, G)
+    lens[0] = 32                                        # whole pages only
+    kinds = [((3, 2), 2, 16, 64, torch.bfloat16), ((2, 1), 1, 8, 20, torch.float32), ((1, 2), 3, 16, 3, torch.bfloat16)]
+    paged = _reorder_case(rng, G, B, lens, (1, 4, 1), kinds, dev)
+    parents = np.stack([rng.permutation(B) for _ in range(G)])
+    again = rng.random((G, B)) < dup
+    parents[again] = rng.integers(-1 if dup < 1 else 0, B, again.sum())
+    if dup == 1.0:
+        parents[0] = 0
+    rows = G * B + 1
+    slots = rng.permutation(rows)[:G * B]
+    states = [torch.randn(rows, 5, 8, 8, device=dev), torch.randn(rows, 3, device=dev), torch.randint(0, 250, (rows, 37), device=dev).to(torch.uint8),
+              torch.randn(rows, 1, device=dev), torch.randn(rows, 40 if many else 9000, device=dev).to(torch.bfloat16)]
+    want_states = [s.clone().cpu().view(torch.int16).numpy() if s.dtype == torch.bfloat16 else s.clone().cpu().numpy() for s in states]
+    want_paged = [((s.clone().cpu().view(torch.int16) if s.dtype == torch.bfloat16 else s.clone().cpu()).numpy(), t.copy(), st) for s, t, st in paged]
+    want_slots, want_tables = plain.reorder(parents, slots, lens, want_states, want_paged)
+    slots_d, tables_d = _i32(slots, dev), [_i32(t, dev) for _, t, _ in paged]
+    got_slots, got_tables = ops.beam_reorder(_i32(parents, dev), slots_d, _i32(lens, dev), states=states, paged=[(s, t, st) for (s, _, st), t in zip(paged, tables_d)])
+    assert np.array_equal(got_slots.cpu().numpy(), want_slots)
+    assert np.array_equal(slots_d.cpu().numpy(), slots)
+    for a, b in zip(got_tables, want_tables):
+        assert np.array_equal(a.cpu().numpy(), b)
+    for s, w in zip(states, want_states):
+        assert np.array_equal((s.cpu().view(torch.int16) if s.dtype == torch.bfloat16 else s.cpu()).numpy(), w)
+    for (s, _, _), (w, _, _) in zip(paged, want_paged):
+        assert np.array_equal((s.cpu().view(torch.int16) if s.dtype == torch.bfloat16 else s.cpu()).numpy(), w)
+
+
+def test_reorder_of_more_states_and_caches_than_a_launch_takes():
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    rng = np.random.default_rng(3)
+    G, B, lens = 2, 3, [21, 5]
+    paged = _reorder_case(rng, G, B, lens, (1,) * 11, [((1, 2), 1, 16, 8, torch.float32)] * 11, dev)
+    parents, slots = np.array([[1, 1, 0], [2, 2, 2]]), np.array([4, 2, 0, 1, 3, 5])
+    states = [torch.randn(7, 4 + i % 3, device=dev) for i in range(130)]
+    want_states = [s.cpu().numpy().copy() for s in states]
+    want_paged = [(s.cpu().numpy().copy(), t.copy(), st) for s, t, st in paged]
+    want_slots, want_tables = plain.reorder(parents, slots, lens, want_states, want_paged)
+    got_slots, got_tables = ops.beam_reorder(_i32(parents, dev), _i32(slots, dev), _i32(lens, dev), states=states, paged=[(s, _i32(t, dev), st) for s, t, st in paged])
+    assert np.array_equal(got_slots.cpu().numpy(), want_slots)
+    assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(got_tables, want_tables))
+    assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(states, want_states))
+    assert all(np.array_equal(s.cpu().numpy(), w) for (s, _, _), (w, _, _) in zip(paged, want_paged))
+
+
+def test_reorder_leaves_alone_what_tables_do_not_name():
+    """Slots and pages outside their storage, negative ones, a context behind the table: nothing is copied there, the rest is."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    kv = torch.randn(1, 2, 4, 1, 16, 8, device=dev)
+    before = kv.clone()
+    state = torch.randn(3, 4, device=dev)
+    held = state.clone()
+    table = _i32([[0, -1], [1, 99]], dev)
+    slots, tables = ops.beam_reorder(_i32([[0, 0]], dev), _i32([0, 7], dev), _i32([20], dev), states=[state], paged=[(kv, table, 1)])
+    assert torch.equal(kv, before) and torch.equal(state, held) and slots.tolist() == [0, 7] and tables[0].tolist() == [[0, -1], [0, 99]]
+    _, tables = ops.beam_reorder(_i32([[1, 1]], dev), _i32([0, 1], dev), _i32([500], dev), states=[state], paged=[(kv, table, 1)])
+    assert torch.equal(kv, before) and torch.equal(state[0], held[1]) and tables[0].tolist() == [[1, 99], [1, 99]]
+
+
+@pytest.mark.parametrize("S,most", [(1, 1), (1, 700), (5, 1), (48, 40), (300, 9), (1100, 2)])
+@pytest.mark.parametrize("grow", [False, True])
+@pytest.mark.parametrize("ps,strides", [(16, (1,)), (8, (1, 4)), (5, (1, 7, 3))])
+def test_step_tables(S, most, grow, ps, strides):
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    rng = np.random.default_rng(S + most + ps)
+    q = rng.integers(0 if S > 1 else 1, most + 1, S)
+    have = np.where(rng.random(S) < 0.2, 0, rng.integers(0, 500, S))
+    rows = rng.permutation(S + 2)[:S]
+    tables, free = [], []
+    for st in strides:
+        had, needs = -(-(have // st) // ps), -(-((have + q) // st) // ps)
+        columns = int(needs.max()) + (1 if st == 1 else 4)
+        ids = rng.permutation(int(needs.sum()) + 9)
+        held = had if grow else needs
+        table, at = np.full((S + 2, columns), -1), 0
+        for s in range(S):
+            table[rows[s], :held[s]] = ids[at:at + held[s]]
+            at += held[s]
+        tables.append(table)
+        free.append(ids[at:] if grow else None)
+    if S > 1:
+        tables[0][rows[0], 0] = -1                        # a page given back by a window
+    for T in sorted({int(q.sum()), int(q.sum()) + 13, max(0, int(q.sum()) - 3)}):
+        columns = [t.shape[1] + (2 if k else 0) for k, t in enumerate(tables)]
+        want_tables = [t.copy() for t in tables]
+        want = plain.step_tables(q, have, want_tables, page_size=ps, num_tokens=T, strides=strides, rows=rows, free=free, columns=columns)
+        dev_tables = [_i32(t, dev) for t in tables]
+        got = ops.step_tables(_i32(q, dev), _i32(have, dev), dev_tables, page_size=ps, num_tokens=T, strides=strides, rows=_i32(rows, dev),
+                              free=[_i32(f, dev) if f is not None else None for f in free], columns=columns)
+        for a, b in zip((*got[:4], *got.block_tables, *got.slot_mappings, *dev_tables), (*want[:4], *want[4], *want[5], *want_tables)):
+            assert np.array_equal(a.cpu().numpy(), b)
+
+
+def test_step_tables_with_too_few_free_pages_and_columns():
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    q, have = [40, 3, 30], [5, 16, 0]
+    tables = [[[7, -1, -1], [8, -1, -1], [-1, -1, -1]]]
+    free = [[3, 4, 5, 6]]                                 # 2 + 1 + 2 are wanted
+    want_t = [np.array(t) for t in tables]
+    want = plain.step_tables(np.array(q), np.array(have), want_t, page_size=16, num_tokens=73, strides=[1], rows=np.arange(3), free=[np.array(free[0])], columns=[2])
+    t = _i32(tables[0], dev)
+    got = ops.step_tables(_i32(q, dev), _i32(have, dev), [t], page_size=16, num_tokens=73, free=[_i32(free[0], dev)], columns=[2])
+    for a, b in zip((*got[:4], *got.block_tables, *got.slot_mappings, t), (*want[:4], *want[4], *want[5], *want_t)):
+        assert np.array_equal(a.cpu().numpy(), b)
+    none = ops.step_tables(_i32([2], dev), _i32([0], dev), [t], page_size=16, num_tokens=2, rows=_i32([9], dev))         # a row that there is not
+    assert none.slot_mappings[0].tolist() == [-1, -1] and none.block_tables[0].tolist() == [[-1] * 3]
+    empty = ops.step_tables(_i32([2], dev), _i32([0], dev), [t], page_size=16, num_tokens=2, rows=_i32([2], dev), free=[_i32([], dev)])
+    assert empty.slot_mappings[0].tolist() == [-1, -1] and t[2].tolist() == [-1, -1, -1]
+
+
+def test_one_step_captured_and_replayed_on_another_stream():
+    """Candidates, advance, reorder and tables as one graph: replays give what the calls gave, with the graph's inputs changed in between."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    G, B, V, ps = 3, 4, 5003, 16
+    logits, scores = torch.empty(G * B, V, device=dev), torch.empty(G, B, device=dev)
+    lengths, done, lens = _i32([3] * G, dev), _i32([0] * G, dev), _i32([37, 20, 64], dev)
+    slots, table = _i32(np.arange(G * B), dev), _i32(np.arange(G * B * 6).reshape(G * B, 6), dev)
+    kv, state = torch.empty(2, 2, G * B * 6, 2, ps, 64, device=dev, dtype=torch.bfloat16), torch.empty(G * B, 1000, device=dev)
+    pool, stop = ops.beam_pool(G, B, dev), _i32([17, 900], dev)
+
+    def fill(seed):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        logits.copy_(torch.randn(G * B, V, device=dev, generator=g) * 3)
+        scores.copy_(-torch.rand(G, B, device=dev, generator=g) * 3)
+        kv.copy_(torch.randn(kv.shape, device=dev, generator=g))
+        state.copy_(torch.randn(state.shape, device=dev, generator=g))
+
+    def step():
+        c = ops.beam_candidates(logits, scores, 12)
+        nxt = ops.beam_advance(*c, pool, lengths, done, beams=B, stop_ids=stop, max_new=20)
+        new_slots, tables = ops.beam_reorder(nxt.parents, slots, lens, states=[state], paged=[(kv, table, 1)])
+        have = lens[:, None].expand(G, B).reshape(-1).contiguous()
+        t = ops.step_tables(torch.ones_like(have), have, tables, page_size=ps, num_tokens=G * B)
+        return (*c, *nxt[:5], *nxt.pool, new_slots, *tables, *t[:4], *t.block_tables, *t.slot_mappings, kv.clone(), state.clone())
+    fill(0)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    side = torch.cuda.Stream()
+    for seed in (1, 2):
+        fill(seed)
+        want = [x.clone() for x in step()]
+        fill(seed)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        for a, b in zip(held, want):
+            assert torch.equal(a, b)
