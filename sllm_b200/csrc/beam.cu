@@ -7,14 +7,14 @@
 // logit, so a beam's own best are those of the largest logits, and no candidate of the search lies outside the `keep` best of its beam:
 //   beam_rows_kernel    a part of a row a block: the part's maximum, its sum of exponentials and its `keep` largest logits, from one pass over the logits;
 //   beam_merge_kernel   a block a search, a warp a beam: the beam's parts joined, then the beams.
-// Exponentials are expf of float32 differences, exact as the logits are; their sums over a row's threads and parts, the logarithm and s are float64 (continuations
+// Exponentials are float32, of float32 differences; their sums over a row's threads and parts, the logarithm and s are float64 (continuations
 // of different beams are compared with each other; of one beam by their logits alone).  s is rounded to float32 once, when it is stored.
 #include "common.cuh"
 
 namespace sllm {
 
 constexpr int BEAM_THREADS = 256, BEAM_KEEP = 128, BEAM_MAX = 32;
-constexpr int BEAM_LOADS = 4;                                   // 16-byte loads a thread and batch
+constexpr int BEAM_VALUES = 16, BEAM_RUN = 8;                   // logits of a thread and batch; batches of a run
 constexpr uint32_t BEAM_MINUS_INFINITY = 0x007fffffu;           // the key of minus infinity: what is not above it offers nothing
 
 // Keys: the logit's bits so that unsigned order is float order, then the token turned around, so that of equal logits the first is the largest key.  0: no key.
@@ -43,6 +43,7 @@ struct BeamPart {
   float max;
 };
 
+// 16 bytes of logits: how many, their values, their largest (a number where there is one), one that is missing, one alone
 template <typename T> struct BeamLoad;
 template <> struct BeamLoad<float> {
   static constexpr int N = 4;
@@ -51,6 +52,15 @@ template <> struct BeamLoad<float> {
     x[1] = __uint_as_float(raw.y);
     x[2] = __uint_as_float(raw.z);
     x[3] = __uint_as_float(raw.w);
+  }
+  static __device__ __forceinline__ float largest(const uint4& raw) {
+    return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+  }
+  template <class F> static __device__ __forceinline__ uint4 gather(const float* p, F there) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = there(i) ? __float_as_uint(p[i]) : 0xff800000u;
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <> struct BeamLoad<__nv_bfloat16> {
@@ -63,11 +73,23 @@ template <> struct BeamLoad<__nv_bfloat16> {
       x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
+  static __device__ __forceinline__ float largest(const uint4& raw) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  template <class F> static __device__ __forceinline__ uint4 gather(const __nv_bfloat16* p, F there) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (there(2 * i) ? (uint32_t)__bfloat16_as_ushort(p[2 * i]) : 0xff80u) | (there(2 * i + 1) ? (uint32_t)__bfloat16_as_ushort(p[2 * i + 1]) : 0xff80u) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
 };
 
 // The list of keys that may belong to the best: what a batch can add (see beam_rows_kernel) beside the `keep` it already holds, and the other half of a
 // filter's ping-pong, which is at most half as long.
-constexpr int BEAM_LIST = BEAM_KEEP * BEAM_LOADS * 8 + BEAM_KEEP, BEAM_OTHER = BEAM_LIST / 2 + BEAM_KEEP;
+constexpr int BEAM_LIST = BEAM_KEEP * BEAM_VALUES + BEAM_KEEP, BEAM_OTHER = BEAM_LIST / 2 + BEAM_KEEP;
 
 struct BeamShared {
   unsigned long long list[BEAM_LIST], other[BEAM_OTHER];
@@ -123,10 +145,13 @@ __device__ int beam_compact(int keep, int log2_lanes, BeamShared& sh) {
     to = t;
     __syncthreads();
   }
-  const unsigned long long me = (int)threadIdx.x < n ? from[threadIdx.x] : 0;
+  unsigned long long me = 0;
   int rank = 0;
+  if ((int)threadIdx.x < n) {
+    me = from[threadIdx.x];
 #pragma unroll 8
-  for (int j = 0; j < n; ++j) rank += from[j] > me;
+    for (int j = 0; j < n; ++j) rank += from[j] > me;
+  }
   __syncthreads();
   if ((int)threadIdx.x < n && rank < keep) sh.list[rank] = me;
   n = n < keep ? n : keep;
@@ -135,11 +160,36 @@ __device__ int beam_compact(int keep, int log2_lanes, BeamShared& sh) {
   return n;
 }
 
-// One part of one row: blockIdx.x = row * splits + part.  What bounds it: reading the logits once.  A batch is BEAM_LOADS 16-byte loads a thread, all in flight
-// together; of a batch only keys that reach the bound, a key that `keep` others are known to reach, enter the list.
+// 2^t, within 2^-22 of it (the hardware's; denormal results are zero)
+__device__ __forceinline__ float exp2_fast(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+
+// two float32 operations an instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+
+// One part of one row: blockIdx.x = row * splits + part.  What bounds it: reading the logits once.  A batch is BEAM_VALUES logits a thread in 16-byte loads, all in flight
+// together, the next batch's under the arithmetic of this one.
+// An exponential is 2^(d log2 e) of the rounded difference d = x - m: off by about 2 |d| + 4 units of 2^-24, of which the sum keeps the mean, |d| being at most
+// ln V on average under the softmax itself.
+// Of a batch only keys that reach the bound, a key that `keep` others are known to reach, enter the list.  The first batch's bound comes from the threads' largest; then BEAM_RUN
+// batches at a time are read without a barrier, every thread adding what reaches the bound, and the list, cut to its `keep` largest, gives the next bound: of logits in no
+// particular order about `keep` a batch in the first run and ever fewer later.  Where a run finds more than the list holds (logits that rise through
+// the row), its batches are read again, one by one, each with a bound of its own.
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const T* logits, int V, int keep, int log2_lanes, int splits, int part_vecs, BeamPart* parts, unsigned long long* keys) {
-  constexpr int N = BeamLoad<T>::N, VALUES = BEAM_LOADS * N;
+__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_rows_kernel(const T* logits, int V, int keep, int log2_lanes, int splits, int part_vecs, BeamPart* parts, unsigned long long* keys) {
+  constexpr int N = BeamLoad<T>::N, LOADS = BEAM_VALUES / N, BATCH = LOADS * BEAM_THREADS;
   extern __shared__ __align__(16) unsigned char beam_smem[];
   BeamShared& sh = *reinterpret_cast<BeamShared*>(beam_smem);
   const int row = blockIdx.x / splits, part = blockIdx.x - row * splits;
@@ -147,89 +197,133 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const T* logits
   // Pieces of 16 bytes of tokens.  Which thread takes which tokens goes by their numbers and not by where the row lies, so that equal rows give equal sums; a row that does not begin
   // on 16 bytes is read an element at a time (from L1 but for the first of a piece).
   const int pieces = (V + N - 1) / N;
-  const bool aligned = (reinterpret_cast<uintptr_t>(x_row) & 15) == 0;
   const int v0 = part * part_vecs, v1 = min(v0 + part_vecs, pieces);
+  const int whole = (reinterpret_cast<uintptr_t>(x_row) & 15) == 0 ? min(v1, V / N) : 0;          // pieces that are read as they lie
   if (threadIdx.x == 0) sh.n = 0;
   unsigned long long bound = (unsigned long long)(BEAM_MINUS_INFINITY + 1) << 32;
-  int n_most = 0;                                  // the list's length at most, the same in all threads
+  float bound_logit = beam_value(BEAM_MINUS_INFINITY + 1);
   float m = -INFINITY, s = 0.f;
-  __syncthreads();
-  pdl_wait();
-  for (int vb = v0; vb < v1; vb += BEAM_LOADS * BEAM_THREADS) {
-    float x[VALUES];
+  auto fetch = [&](int vb, uint4* raw) {
+    if (vb + BATCH <= whole) {
+      const uint4* p = reinterpret_cast<const uint4*>(x_row) + vb + threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < BEAM_LOADS; ++u) {
-      const int v = vb + u * BEAM_THREADS + threadIdx.x, first = v * N;
-      if (aligned && v < v1 && first + N <= V) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(x_row + first);
-        BeamLoad<T>::unpack(raw, x + u * N);
-      } else {
+      for (int u = 0; u < LOADS; ++u) raw[u] = p[u * BEAM_THREADS];
+    } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[u * N + i] = v < v1 && first + i < V ? to_f32(x_row[first + i]) : -INFINITY;
+      for (int u = 0; u < LOADS; ++u) {
+        const int v = vb + u * BEAM_THREADS + threadIdx.x, first = v * N;
+        if (v < whole) raw[u] = *reinterpret_cast<const uint4*>(x_row + first);
+        else raw[u] = BeamLoad<T>::gather(x_row + first, [&](int i) { return v < v1 && first + i < V; });
       }
     }
+  };
+  // values and the largest of them (a number where there is one)
+  auto open = [&](const uint4* raw, float* x) {
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < VALUES; ++i) {
-      x[i] = x[i] == x[i] ? x[i] + 0.0f : -INFINITY;          // not a number: no candidate; minus zero is zero
-      top = fmaxf(top, x[i]);
+    for (int u = 0; u < LOADS; ++u) {
+      BeamLoad<T>::unpack(raw[u], x + u * N);
+      top = fmaxf(top, BeamLoad<T>::largest(raw[u]));
     }
+    return top;
+  };
+  auto add_up = [&](const float* x, float top) {
     if (top > m) {
-      s *= expf(m - top);                          // (minus infinity first: times zero)
+      s *= exp2_fast((m - top) * 1.4426950408889634f);                  // (minus infinity first: times zero)
       m = top;
     }
     if (m > -INFINITY) {
-      float p0 = 0.f, p1 = 0.f;
-      if (m < INFINITY) {
+      const float2 by = make_float2(-m, -m), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+      float2 p[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-        for (int i = 0; i < VALUES; i += 2) {
-          p0 += expf(x[i] - m);
-          p1 += expf(x[i + 1] - m);
-        }
-      } else {                                     // all of the mass lies on the infinite ones
-        for (int i = 0; i < VALUES; ++i) p0 += x[i] == m ? 1.f : 0.f;
+      for (int i = 0; i < BEAM_VALUES; i += 2) {
+        const float2 t = mul2(add2(make_float2(x[i], x[i + 1]), by), log2e);
+        p[(i >> 1) & 1] = add2(p[(i >> 1) & 1], make_float2(exp2_fast(t.x), exp2_fast(t.y)));
       }
-      s += p0 + p1;
-    }
-    // the list
-    const bool reaches = beam_order(top) >= (uint32_t)(bound >> 32) && top > -INFINITY;
-    const int flagged = __syncthreads_count(reaches);
-    if (flagged == 0) continue;
-    if (n_most + flagged * VALUES > BEAM_LIST) {
-      n_most = sh.n;                               // (nobody adds before the next barrier)
-      __syncthreads();
-      if (n_most + flagged * VALUES > BEAM_LIST) {
-        if (n_most > 0) {
-          n_most = beam_compact(keep, log2_lanes, sh);
-          if (n_most == keep) bound = bound > sh.list[keep - 1] ? bound : sh.list[keep - 1];
+      float add = (p[0].x + p[0].y) + (p[1].x + p[1].y);
+      // (asked of the bits: the compiler takes what the exponential's asm gives for numbers and leaves `!(add >= 0.f)` out)
+      if ((__float_as_uint(add) & 0x7fffffffu) > 0x7f800000u) {         // a logit that is none, which counts for nothing, or an infinite one, on which all of the mass lies
+        add = 0.f;
+#pragma unroll
+        for (int i = 0; i < BEAM_VALUES; ++i) {
+          if (x[i] == m) add += 1.f;
+          else if (x[i] < m && m < INFINITY) add += exp2_fast((x[i] - m) * 1.4426950408889634f);
         }
-        // of this batch: keys from the keep-th largest of the groups' largest on, which are those of fewer than `keep` groups and one more
-        unsigned long long best = 0;
+      }
+      s += add;
+    }
+  };
+  // a logit's key, 0 where it offers nothing; minus zero is zero
+  auto key_of = [&](float f, int vb, int i) {
+    f += 0.0f;
+    return f > -INFINITY ? beam_key(f, (vb + (i / N) * BEAM_THREADS + (int)threadIdx.x) * N + i % N) : 0ull;
+  };
+  auto append = [&](const float* x, float top, int vb) {
+    if (top >= bound_logit) {
 #pragma unroll
-        for (int u = 0; u < BEAM_LOADS; ++u)
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const unsigned long long k = beam_key(x[u * N + i], (vb + u * BEAM_THREADS + (int)threadIdx.x) * N + i);
-            if (x[u * N + i] > -INFINITY && k > best) best = k;
+      for (int i = 0; i < BEAM_VALUES; ++i)
+        if (x[i] >= bound_logit) {
+          const unsigned long long k = key_of(x[i], vb, i);
+          if (k >= bound) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < BEAM_LIST) sh.list[at] = k;
           }
-        const unsigned long long b = beam_group_bound(best, log2_lanes, keep, sh);
-        bound = bound > b ? bound : b;
-        n_most = BEAM_LIST;                        // (looked up again when it matters)
-      } else {
-        n_most += flagged * VALUES;
-      }
-    } else {
-      n_most += flagged * VALUES;
-    }
-    if (reaches) {
-#pragma unroll
-      for (int u = 0; u < BEAM_LOADS; ++u)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (!(x[u * N + i] > -INFINITY)) continue;
-          const unsigned long long k = beam_key(x[u * N + i], (vb + u * BEAM_THREADS + (int)threadIdx.x) * N + i);
-          if (k >= bound) sh.list[atomicAdd(&sh.n, 1)] = k;
         }
+    }
+  };
+  auto raise = [&](unsigned long long b) {
+    bound = bound > b ? bound : b;
+    bound_logit = beam_value((uint32_t)(bound >> 32));
+  };
+  auto cut = [&]() {
+    if (beam_compact(keep, log2_lanes, sh) == keep) raise(sh.list[keep - 1]);
+    __syncthreads();
+  };
+  // One batch behind a barrier: at most `keep` keys are in the list, and those of this batch from the keep-th largest of the groups' largest on join them, which are those of
+  // fewer than `keep` groups and one more.
+  auto add_batch = [&](const float* x, float top, int vb) {
+    int at = 0;
+#pragma unroll
+    for (int i = BEAM_VALUES - 1; i >= 0; --i) at = x[i] == top ? i : at;          // the first of the largest (of two zeros either will do: both reach the bound then)
+    raise(beam_group_bound(key_of(top, vb, at), log2_lanes, keep, sh));
+    append(x, top, vb);
+  };
+  uint4 next[LOADS];
+  float x[BEAM_VALUES];
+  __syncthreads();
+  pdl_wait();
+  fetch(v0, next);
+  {
+    const float top = open(next, x);
+    if (v0 + BATCH < v1) fetch(v0 + BATCH, next);
+    add_up(x, top);
+    add_batch(x, top, v0);
+  }
+  int vb = v0 + BATCH;
+  while (vb < v1) {
+    __syncthreads();
+    const int held = sh.n, run = vb, end = min(vb + BEAM_RUN * BATCH, v1);
+    __syncthreads();
+    for (; vb < end; vb += BATCH) {
+      const float top = open(next, x);
+      if (vb + BATCH < v1) fetch(vb + BATCH, next);
+      add_up(x, top);
+      append(x, top, vb);
+    }
+    __syncthreads();
+    const int n = sh.n;
+    if (n > BEAM_LIST) {
+      __syncthreads();
+      if (threadIdx.x == 0) sh.n = held;
+      cut();
+      uint4 raw[LOADS];
+      for (int again = run; again < end; again += BATCH) {
+        fetch(again, raw);
+        add_batch(x, open(raw, x), again);
+        cut();
+      }
+    } else if (n > 4 * keep) {
+      cut();
     }
   }
   pdl_launch_dependents();
@@ -244,91 +338,107 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const T* logits
     sh.red_s[warp] = ws;
   }
   const int n = beam_compact(keep, log2_lanes, sh);
-  if (threadIdx.x == 0) {
-    float am = sh.red_m[0];
-    for (int w = 1; w < BEAM_THREADS / 32; ++w) am = fmaxf(am, sh.red_m[w]);
-    double as = 0.0;
-    for (int w = 0; w < BEAM_THREADS / 32; ++w)
-      if (sh.red_m[w] > -INFINITY && (am < INFINITY || sh.red_m[w] == am)) as += sh.red_s[w] * (sh.red_m[w] == am ? 1.0 : exp((double)sh.red_m[w] - (double)am));
-    parts[blockIdx.x] = BeamPart{as, am};
+  if (warp == 0) {
+    const float wmax = lane < BEAM_THREADS / 32 ? sh.red_m[lane] : -INFINITY, all = warp_max(wmax);
+    double sum = 0.0;
+    if (wmax > -INFINITY && (all < INFINITY || wmax == all)) sum = sh.red_s[lane] * (wmax == all ? 1.0 : exp((double)wmax - (double)all));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) parts[blockIdx.x] = BeamPart{sum, all};
   }
   for (int i = threadIdx.x; i < keep; i += BEAM_THREADS) keys[(size_t)blockIdx.x * keep + i] = i < n ? sh.list[i] : 0ull;
 }
 
-// A search: warp b joins the parts of beam b's row, then the first warp joins the beams.  Every step of a join takes the largest of the lists' heads.
+// A search: warp b joins the parts of beam b's row, then the first warp joins the beams.  Every step of a join takes the largest of the lists' heads, one a lane; the key behind a head
+// is loaded before the head goes.
+struct BeamHead {
+  const unsigned long long* list;
+  int at, n;
+  unsigned long long head, behind;
+  __device__ __forceinline__ BeamHead(const unsigned long long* l, int length) : list(l), at(2), n(length) {
+    head = n > 0 ? list[0] : 0ull;
+    behind = n > 1 ? list[1] : 0ull;
+  }
+  __device__ __forceinline__ void pop() {
+    head = behind;
+    behind = at < n ? list[at] : 0ull;
+    ++at;
+  }
+};
+
 __global__ void beam_merge_kernel(const float* scores, const BeamPart* parts, const unsigned long long* keys, int B, int keep, int splits, float* out_score, int* out_parent,
                                   int* out_token) {
   extern __shared__ __align__(16) unsigned char beam_smem[];
   unsigned long long* lists = reinterpret_cast<unsigned long long*>(beam_smem);        // [B][splits][keep]: a beam's parts
-  unsigned long long* head_score = lists + (size_t)B * splits * keep;                  // [B][keep]: a beam's scores, joined
-  int* best_token = reinterpret_cast<int*>(head_score + B * keep);                     // [B][keep]
+  unsigned long long* merged = lists + (size_t)B * splits * keep;                      // [B][keep]: a beam's keys joined, then its scores
+  int* best_token = reinterpret_cast<int*>(merged + B * keep);                         // [B][keep]
   pdl_launch_dependents();
   pdl_wait();
   const int g = blockIdx.x, b = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t row = (size_t)g * B + b;
-  const float score = scores[row];
   {
-    unsigned long long* mine = lists + (size_t)b * splits * keep;
+    const float score = scores[row];
+    unsigned long long *mine = lists + (size_t)b * splits * keep, *joined = merged + b * keep;
     const unsigned long long* src = keys + row * splits * keep;
+    const BeamPart part = lane < splits ? parts[row * splits + lane] : BeamPart{0.0, -INFINITY};
+#pragma unroll 4
     for (int i = lane; i < splits * keep; i += 32) mine[i] = src[i];
-    float top = -INFINITY;
-    for (int p = lane; p < splits; p += 32) top = fmaxf(top, parts[row * splits + p].max);
-    top = warp_max(top);
+    const float top = warp_max(part.max);
     double sum = 0.0;
-    for (int p = lane; p < splits; p += 32) {
-      const BeamPart q = parts[row * splits + p];
-      if (q.max == top) sum += q.sum;
-      else if (top < INFINITY && q.max > -INFINITY) sum += q.sum * exp((double)q.max - (double)top);
-    }
+    if (part.max > -INFINITY && (top < INFINITY || part.max == top)) sum = part.max == top ? part.sum : part.sum * exp((double)part.max - (double)top);
+    if (splits > 1) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double lse = log(sum);
-    const bool alive = score > -INFINITY && top > -INFINITY;
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    } else {
+      sum = __shfl_sync(0xffffffffu, sum, 0);
+    }
     __syncwarp();
     int n = 0;
-    if (alive) {                                    // lane l walks the l-th part's list
-      int at = 0;
-      unsigned long long head = lane < splits ? mine[lane * keep] : 0ull;
+    if (splits > 1) {                               // lane l walks the l-th part's list
+      BeamHead h(mine + lane * keep, lane < splits ? keep : 0);
       for (; n < keep; ++n) {
-        const unsigned long long best = warp_max_key(head);
+        const unsigned long long best = warp_max_key(h.head);
         if (best == 0) break;
-        if (lane == 0) {
-          const float x = beam_value((uint32_t)(best >> 32));
-          const double d = x == top ? 0.0 : (double)x - (double)top;
-          const double v = (double)score + (d - lse);
-          head_score[b * keep + n] = v > -INFINITY ? order_double(v) : 0ull;
-          best_token[b * keep + n] = (int)~(uint32_t)best;
-        }
-        if (head == best) {
-          ++at;
-          head = at < keep ? mine[lane * keep + at] : 0ull;
+        if (h.head == best) {
+          joined[n] = best;
+          h.pop();
         }
       }
+      __syncwarp();
+    } else {
+      joined = mine;
+      n = keep;
     }
-    for (int i = n + lane; i < keep; i += 32) head_score[b * keep + i] = 0;
+    const bool alive = score > -INFINITY && top > -INFINITY;
+    const double lse = log(sum);
+    for (int i = lane; i < keep; i += 32) {
+      const unsigned long long k = i < n && alive ? joined[i] : 0ull;
+      const float x = beam_value((uint32_t)(k >> 32));
+      const double v = (double)score + ((x == top ? 0.0 : (double)x - (double)top) - lse);
+      merged[b * keep + i] = k != 0 && v > -INFINITY ? order_double(v) : 0ull;
+      best_token[b * keep + i] = (int)~(uint32_t)k;
+    }
   }
   __syncthreads();
   if (b != 0) return;
-  int at = 0;
-  unsigned long long head = lane < B ? head_score[lane * keep] : 0ull;
+  BeamHead h(merged + lane * keep, lane < B ? keep : 0);
   for (int n = 0; n < keep; ++n) {
-    const unsigned long long best = warp_max_key(head);
+    const unsigned long long best = warp_max_key(h.head);
     const size_t o = (size_t)g * keep + n;
     if (best == 0) {
-      if (lane == 0) {
-        out_score[o] = -INFINITY;
-        out_parent[o] = -1;
-        out_token[o] = -1;
+      for (int i = n + lane; i < keep; i += 32) {
+        out_score[(size_t)g * keep + i] = -INFINITY;
+        out_parent[(size_t)g * keep + i] = -1;
+        out_token[(size_t)g * keep + i] = -1;
       }
-      continue;
+      break;
     }
-    const int who = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;       // of equal scores the first beam's
+    const int who = __ffs(__ballot_sync(0xffffffffu, h.head == best)) - 1;     // of equal scores the first beam's
     if (lane == who) {
       out_score[o] = (float)double_of(best);
       out_parent[o] = lane;
-      out_token[o] = best_token[lane * keep + at];
-      ++at;
-      head = at < keep ? head_score[lane * keep + at] : 0ull;
+      out_token[o] = best_token[lane * keep + h.at - 2];
+      h.pop();
     }
   }
 }
@@ -343,8 +453,6 @@ struct BeamPool {
   float* score;
   int *length, *parent, *token;
 };
-
-__device__ __forceinline__ float beam_norm(float s, int n, double power) { return (float)((double)s / pow((double)n, power)); }
 
 __global__ void __launch_bounds__(32) beam_advance_kernel(const float* c_score, const int* c_parent, const int* c_token, int keep, int beams, int W, const float* p_score,
                                                           const int* p_length, const int* p_parent, const int* p_token, const int* lengths, const int* done, const int* stop_ids,
@@ -370,14 +478,14 @@ __global__ void __launch_bounds__(32) beam_advance_kernel(const float* c_score, 
   const int before = lengths[g], n = before + 1;
   bool over = was_done;
   constexpr int PER = BEAM_KEEP / 32;
-  float cs[PER];
+  float cs[PER], norm[PER];
   int cp[PER], ct[PER], place[PER];              // place: among those that go on, -1: not one of them
   int live = 0;
   float lead = -INFINITY;
   if (!was_done) {
     unsigned stop_mask[PER];
-    auto enter = [&](float s, int parent, int token) {        // uniform
-      const float v = beam_norm(s, n, power);
+    const double length = pow((double)n, power), reach = pow((double)(power >= 0.0 ? max_new : n + 1), power);
+    auto enter = [&](float v, int parent, int token) {        // uniform
       const int at = __popc(__ballot_sync(full, lane < W && ps >= v));
       const float us = __shfl_up_sync(full, ps, 1);
       const int ul = __shfl_up_sync(full, pl, 1), up = __shfl_up_sync(full, pp, 1), ut = __shfl_up_sync(full, pt, 1);
@@ -395,6 +503,7 @@ __global__ void __launch_bounds__(32) beam_advance_kernel(const float* c_score, 
       cs[j] = in ? c_score[(size_t)g * keep + r] : -INFINITY;
       cp[j] = in ? c_parent[(size_t)g * keep + r] : -1;
       ct[j] = in ? c_token[(size_t)g * keep + r] : -1;
+      norm[j] = (float)((double)cs[j] / length);
       bool stop = false;
       for (int k = 0; k < stops; ++k) stop |= stop_ids[k] == ct[j];
       const bool there = cs[j] > -INFINITY;
@@ -411,20 +520,20 @@ __global__ void __launch_bounds__(32) beam_advance_kernel(const float* c_score, 
     for (int j = 0; j < PER; ++j)
       for (unsigned mask = stop_mask[j]; mask; mask &= mask - 1) {
         const int l = __ffs(mask) - 1;
-        enter(__shfl_sync(full, cs[j], l), __shfl_sync(full, cp[j], l), __shfl_sync(full, ct[j], l));
+        enter(__shfl_sync(full, norm[j], l), __shfl_sync(full, cp[j], l), __shfl_sync(full, ct[j], l));
       }
     if (n >= max_new) {
 #pragma unroll
       for (int j = 0; j < PER; ++j)
         for (unsigned mask = __ballot_sync(full, place[j] >= 0); mask; mask &= mask - 1) {
           const int l = __ffs(mask) - 1;
-          enter(__shfl_sync(full, cs[j], l), __shfl_sync(full, cp[j], l), __shfl_sync(full, ct[j], l));
+          enter(__shfl_sync(full, norm[j], l), __shfl_sync(full, cp[j], l), __shfl_sync(full, ct[j], l));
         }
       over = true;
     }
     const float last = __shfl_sync(full, ps, W - 1);
     if (live == 0) over = true;
-    else if (last > -INFINITY && beam_norm(lead, power >= 0.0 ? max_new : n + 1, power) <= last) over = true;
+    else if (last > -INFINITY && (float)((double)lead / reach) <= last) over = true;
   }
   // the next beams: those that go on, in order; the others of them idle (parent -1), or all of them where the search is over
   if (lane < beams && (over || lane >= live)) {

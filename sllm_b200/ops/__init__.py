@@ -2628,17 +2628,18 @@ BeamStep = namedtuple("BeamStep", "scores parents tokens lengths done pool")
 StepTables = namedtuple("StepTables", "q_start ctx_len positions seq_of_token block_tables slot_mappings")
 
 
-def _one_device(what: str, *tensors) -> None:
-    """All on the current device: the launch goes to its current stream."""
+def _here(what: str, *tensors) -> None:
+    """`_chk`, and all on the current device: the launch goes to its current stream."""
     index = _current_device() if _current_device is not None else torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != index:
+        if t is not None and (t.get_device() != index or not t.is_contiguous()):
+            _chk(t)
             raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{index}")
 
 
 def _typed(what: str, dtype, shape, *tensors) -> None:
     for t in tensors:
-        if t.dtype != dtype or tuple(t.shape) != shape:
+        if t.dtype is not dtype or t.shape != shape:
             raise KernelError(f"{what}: {t.dtype} {tuple(t.shape)}, not {dtype} {shape}")
 
 
@@ -2650,17 +2651,16 @@ def beam_candidates(logits: torch.Tensor, scores: torch.Tensor, keep: int):
 
     A beam whose score is minus infinity or not a number takes no part, nor does a logit that is; where there are fewer
     candidates the rest is minus infinity, beam -1, token -1.  At most 32 beams and 128 candidates a search."""
-    _chk(logits, scores)
-    _one_device("beam_candidates", logits, scores)
+    _here("beam_candidates", logits, scores)
     if logits.dim() != 2 or scores.dim() != 2 or scores.dtype != torch.float32 or logits.shape[0] != scores.numel():
         raise KernelError(f"beam_candidates: logits {tuple(logits.shape)} and {scores.dtype} scores {tuple(scores.shape)}, not [G*B, V] and float32 [G, B]")
     (G, B), V, keep, dt = scores.shape, logits.shape[1], int(keep), _dt(logits)
     if not 1 <= B <= MAX_BEAMS or not 1 <= keep <= MAX_CANDIDATES or V < 1:
         raise KernelError(f"beam_candidates: {B} beams (1 to {MAX_BEAMS}), {keep} candidates (1 to {MAX_CANDIDATES}), {V} logits")
     dev = logits.device
-    out_s = torch.empty((G, keep), dtype=torch.float32, device=dev)
-    out_i = torch.empty((2, G, keep), dtype=torch.int32, device=dev)
-    parents, tokens = out_i.unbind(0)
+    out_s = torch.empty(G, keep, dtype=torch.float32, device=dev)
+    parents = torch.empty(G, keep, dtype=torch.int32, device=dev)
+    tokens = torch.empty_like(parents)
     if G == 0:
         return out_s, parents, tokens
     splits = lib().sllm_beam_splits(G, B, V, keep)
@@ -2691,9 +2691,7 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     its pool and length.  ``out``: a `BeamStep` of tensors to write, the inputs' own among them.  At most 32 beams, a pool of 32 and 128 candidates."""
     if out is None:
         out = BeamStep(*(None,) * 5, BeamPool(*(None,) * 4))
-    given = (scores, parents, tokens, *pool, lengths, done)
-    _chk(*given, stop_ids, *out[:5], *out.pool)
-    _one_device("beam_advance", *given, stop_ids, *out[:5], *out.pool)
+    _here("beam_advance", scores, parents, tokens, *pool, lengths, done, stop_ids, *out[:5], *out.pool)
     if scores.dim() != 2 or pool.scores.dim() != 2:
         raise KernelError("beam_advance: candidates [G, keep] and a pool [G, W]")
     (G, keep), W, beams, max_new, power = scores.shape, pool.scores.shape[1], int(beams), int(max_new), float(length_penalty)
@@ -2708,15 +2706,18 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     if stop_ids is not None and stop_ids.dtype != torch.int32:
         raise KernelError("beam_advance: stop ids are int32")
     dev = scores.device
-    shapes = BeamStep(*(((G, beams), torch.float32),), *((((G, beams), torch.int32),) * 2), *((((G,), torch.int32),) * 2),
-                      (((G, W), torch.float32),) + (((G, W), torch.int32),) * 3)
 
-    def place(t, what):
+    def place(t, what, dtype, shape, like):
         if t is None:
-            return torch.empty(what[0], dtype=what[1], device=dev)
-        _typed("beam_advance: out", what[1], what[0], t)
+            return torch.empty(*shape, dtype=dtype, device=dev) if like is None else torch.empty_like(like)
+        _typed("beam_advance: out." + what, dtype, shape, t)
         return t
-    res = BeamStep(*(place(t, w) for t, w in zip(out[:5], shapes[:5])), BeamPool(*(place(t, w) for t, w in zip(out.pool, shapes.pool))))
+    i32, f32 = torch.int32, torch.float32
+    nxt_parents = place(out.parents, "parents", i32, (G, beams), None)
+    res = BeamStep(place(out.scores, "scores", f32, (G, beams), None), nxt_parents, place(out.tokens, "tokens", i32, (G, beams), nxt_parents),
+                   place(out.lengths, "lengths", i32, (G,), lengths), place(out.done, "done", i32, (G,), done),
+                   BeamPool(place(out.pool.scores, "pool.scores", f32, (G, W), pool.scores), place(out.pool.lengths, "pool.lengths", i32, (G, W), pool.lengths),
+                            place(out.pool.parents, "pool.parents", i32, (G, W), pool.parents), place(out.pool.tokens, "pool.tokens", i32, (G, W), pool.tokens)))
     if G:
         call("sllm_beam_advance", _p(scores), _p(parents), _p(tokens), G, keep, beams, W, *(_p(t) for t in pool), _p(lengths), _p(done),
              _p(stop_ids), stop_ids.numel() if stop_ids is not None else 0, max_new, ctypes.byref(ctypes.c_double(power)),
@@ -2736,8 +2737,7 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
     Returns ``(new slots, [new block tables])``; ``out`` is such a pair of tensors to write (others than those read).  At most 32 beams a search, 2,048 in all."""
     states, paged = list(states), [(s, t, int(st)) for s, t, st in paged]
     new_slots, tables = out if out is not None else (None, [None] * len(paged))
-    _chk(parents, slots, lens, *states, *(x for p in paged for x in p[:2]), new_slots, *tables)
-    _one_device("beam_reorder", parents, slots, lens, *states, *(x for p in paged for x in p[:2]), new_slots, *tables)
+    _here("beam_reorder", parents, slots, lens, *states, *(x for p in paged for x in p[:2]), new_slots, *tables)
     if parents.dim() != 2 or len(tables) != len(paged):
         raise KernelError(f"beam_reorder: parents {tuple(parents.shape)}, not [G, B], or {len(tables)} tables for {len(paged)} caches")
     G, B = parents.shape
@@ -2808,8 +2808,7 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
     if len(strides) != n or len(free) != n or len(columns) != n or n > 8:
         raise KernelError(f"step_tables: {n} groups (8 at most), {len(strides)} strides, {len(free)} lists of free pages, {len(columns)} numbers of columns")
     flat = (q_lens, have, rows, *page_tables, *free) + ((*out[:4], *out.block_tables, *out.slot_mappings) if out is not None else ())
-    _chk(*flat)
-    _one_device("step_tables", *flat)
+    _here("step_tables", *flat)
     S = q_lens.numel()
     if S < 1 or T < 0 or page_size < 1 or any(s < 1 for s in strides):
         raise KernelError(f"step_tables: {S} requests, {T} tokens, pages of {page_size}, strides {strides}")
@@ -2827,10 +2826,9 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
         raise KernelError(f"step_tables: {columns} columns")
     if out is None:
         dev = q_lens.device
-        per_seq = torch.empty(2 * S + 1, dtype=torch.int32, device=dev)
-        per_token = torch.empty((2 + n, T), dtype=torch.int32, device=dev).unbind(0)
-        out = StepTables(per_seq[:S + 1], per_seq[S + 1:], per_token[0], per_token[1],
-                         tuple(torch.empty((S, c), dtype=torch.int32, device=dev) for c in columns), tuple(per_token[2:]))
+        positions = torch.empty(T, dtype=torch.int32, device=dev)
+        out = StepTables(torch.empty(S + 1, dtype=torch.int32, device=dev), torch.empty_like(have), positions, torch.empty_like(positions),
+                         tuple(torch.empty(S, c, dtype=torch.int32, device=dev) for c in columns), tuple(torch.empty_like(positions) for _ in page_tables))
     else:
         _typed("step_tables: out.q_start", torch.int32, (S + 1,), out.q_start)
         _typed("step_tables: out.ctx_len", torch.int32, (S,), out.ctx_len)
