@@ -14,7 +14,7 @@
 namespace sllm {
 
 constexpr int BEAM_THREADS = 256, BEAM_KEEP = 128, BEAM_MAX = 32;
-constexpr int BEAM_VALUES = 16, BEAM_RUN = 8;                   // logits of a thread and batch; batches of a run
+constexpr int BEAM_VALUES = 16;                                 // logits of a thread and batch
 constexpr uint32_t BEAM_MINUS_INFINITY = 0x007fffffu;           // the key of minus infinity: what is not above it offers nothing
 
 // Keys: the logit's bits so that unsigned order is float order, then the token turned around, so that of equal logits the first is the largest key.  0: no key.
@@ -87,17 +87,17 @@ template <> struct BeamLoad<__nv_bfloat16> {
   }
 };
 
-// The list of keys that may belong to the best: what a batch can add (see beam_rows_kernel) beside the `keep` it already holds, and the other half of a
-// filter's ping-pong, which is at most half as long.
+// LIST: keys that may belong to the best, what a batch can add (see beam_rows_kernel) beside the `keep` already held at the least; OTHER: the other half of a filter's ping-pong, what
+// a pass over a full list can leave.
 constexpr int BEAM_LIST = BEAM_KEEP * BEAM_VALUES + BEAM_KEEP, BEAM_OTHER = BEAM_LIST / 2 + BEAM_KEEP;
 
 struct BeamShared {
   unsigned long long list[BEAM_LIST], other[BEAM_OTHER];
   unsigned long long group[BEAM_THREADS];
   unsigned long long bound;
-  int n;
-  float red_m[BEAM_THREADS / 32];
   double red_s[BEAM_THREADS / 32];
+  float red_m[BEAM_THREADS / 32];
+  int n;
 };
 
 // The keep-th largest of the groups' largest keys, known to all threads: `keep` keys at least are no smaller.  0 where fewer than `keep` groups have a key.
@@ -124,8 +124,8 @@ __device__ unsigned long long beam_group_bound(unsigned long long mine, int log2
   return b;
 }
 
-// The keys sh.list[0, sh.n) become their `keep` largest, sorted; returns how many there are.  Filters by the groups' bound until 256 at most are left (each pass leaves at most
-// (keep - 1) groups' keys and one, under half of them), then every key finds its place.
+// The keys sh.list[0, sh.n) become their `keep` largest, sorted; returns how many there are.  Filters by the groups' bound until no more than the threads are left (each pass
+// leaves at most (keep - 1) groups' keys and one, about half of them), then every key finds its place.
 __device__ int beam_compact(int keep, int log2_lanes, BeamShared& sh) {
   __syncthreads();
   int n = sh.n;
@@ -173,22 +173,24 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
   return r;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
   return r;
 }
 
 // One part of one row: blockIdx.x = row * splits + part.  What bounds it: reading the logits once.  A batch is BEAM_VALUES logits a thread in 16-byte loads, all in flight
 // together, the next batch's under the arithmetic of this one.
-// An exponential is 2^(d log2 e) of the rounded difference d = x - m: off by about 2 |d| + 4 units of 2^-24, of which the sum keeps the mean, |d| being at most
-// ln V on average under the softmax itself.
-// Of a batch only keys that reach the bound, a key that `keep` others are known to reach, enter the list.  The first batch's bound comes from the threads' largest; then BEAM_RUN
-// batches at a time are read without a barrier, every thread adding what reaches the bound, and the list, cut to its `keep` largest, gives the next bound: of logits in no
-// particular order about `keep` a batch in the first run and ever fewer later.  Where a run finds more than the list holds (logits that rise through
+// An exponential is 2^(x log2 e - c) in one rounding of the exponent: off by about |x - m| + 4 units of 2^-24, of which the sum keeps the mean, |x - m| being at most ln V on
+// average under the softmax itself.
+// Of a batch only keys that reach the bound, a key that `keep` others are known to reach, enter the list.  The first batch's bound comes from the threads' largest; then runs
+// of 3, 12, 48, ... batches are read without a barrier, every thread adding what reaches the bound, and the list, cut to its `keep` largest, gives the next bound: of logits in
+// no particular order three times `keep` a run.  Where a run finds more than the list holds (logits that rise through
 // the row), its batches are read again, one by one, each with a bound of its own.
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_rows_kernel(const T* logits, int V, int keep, int log2_lanes, int splits, int part_vecs, BeamPart* parts, unsigned long long* keys) {
+__global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_kernel(const T* logits, int V, int keep, int log2_lanes, int splits, int part_vecs, BeamPart* parts, unsigned long long* keys) {
   constexpr int N = BeamLoad<T>::N, LOADS = BEAM_VALUES / N, BATCH = LOADS * BEAM_THREADS;
   extern __shared__ __align__(16) unsigned char beam_smem[];
   BeamShared& sh = *reinterpret_cast<BeamShared*>(beam_smem);
@@ -227,28 +229,38 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_rows_kernel(const T* log
     }
     return top;
   };
+  // s: the sum of 2^(x log2 e - c) with c = m log2 e rounded; what the rounding left, `rest`, is taken out when m moves and at the end.  Where m log2 e has no place in
+  // float32 (an infinite m, rows at the type's ends), c is not a number and every batch goes the long way.
+  const float log2e = 1.4426950408889634f;
+  float c = 0.f, rest = 0.f;
   auto add_up = [&](const float* x, float top) {
     if (top > m) {
-      s *= exp2_fast((m - top) * 1.4426950408889634f);                  // (minus infinity first: times zero)
+      const float to = top * log2e;
+      const bool in = fabsf(to) < 1e38f;
+      const float left = in ? fmaf(top, log2e, -to) : 0.f;
+      if (m > -INFINITY) s *= exp2_fast((m - top) * log2e) * exp2_fast(left - rest);
       m = top;
+      c = in ? to : __uint_as_float(0x7fffffffu);
+      rest = left;
     }
     if (m > -INFINITY) {
-      const float2 by = make_float2(-m, -m), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+      const float2 by = make_float2(-c, -c), factor = make_float2(log2e, log2e);
       float2 p[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (int i = 0; i < BEAM_VALUES; i += 2) {
-        const float2 t = mul2(add2(make_float2(x[i], x[i + 1]), by), log2e);
+        const float2 t = fma2(make_float2(x[i], x[i + 1]), factor, by);
         p[(i >> 1) & 1] = add2(p[(i >> 1) & 1], make_float2(exp2_fast(t.x), exp2_fast(t.y)));
       }
       float add = (p[0].x + p[0].y) + (p[1].x + p[1].y);
-      // (asked of the bits: the compiler takes what the exponential's asm gives for numbers and leaves `!(add >= 0.f)` out)
-      if ((__float_as_uint(add) & 0x7fffffffu) > 0x7f800000u) {         // a logit that is none, which counts for nothing, or an infinite one, on which all of the mass lies
+      // (asked of the bits: the compiler takes what the exponential's asm gives for numbers and leaves `add != add` out)
+      if ((__float_as_uint(add) & 0x7fffffffu) >= 0x7f800000u) {        // a logit that is none, which counts for nothing, or an infinite one, on which all of the mass lies
         add = 0.f;
 #pragma unroll
         for (int i = 0; i < BEAM_VALUES; ++i) {
           if (x[i] == m) add += 1.f;
-          else if (x[i] < m && m < INFINITY) add += exp2_fast((x[i] - m) * 1.4426950408889634f);
+          else if (x[i] < m && m < INFINITY) add += exp2_fast((x[i] - m) * log2e);
         }
+        add *= exp2_fast(rest);
       }
       s += add;
     }
@@ -300,9 +312,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_rows_kernel(const T* log
     add_batch(x, top, v0);
   }
   int vb = v0 + BATCH;
-  while (vb < v1) {
+  for (int batches = 3; vb < v1; batches = min(4 * batches, 1 << 20)) {
     __syncthreads();
-    const int held = sh.n, run = vb, end = min(vb + BEAM_RUN * BATCH, v1);
+    const int held = sh.n, run = vb, end = min(vb + batches * BATCH, v1);
     __syncthreads();
     for (; vb < end; vb += BATCH) {
       const float top = open(next, x);
@@ -322,13 +334,14 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_rows_kernel(const T* log
         add_batch(x, open(raw, x), again);
         cut();
       }
-    } else if (n > 4 * keep) {
+    } else if (n > keep) {
       cut();
     }
   }
   pdl_launch_dependents();
   // the part's maximum and sum
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  s *= exp2_fast(-rest);
   const float wm = warp_max(m);
   double ws = (m > -INFINITY && (wm < INFINITY || m == wm)) ? (double)s * (m == wm ? 1.0 : exp((double)m - (double)wm)) : 0.0;
 #pragma unroll
@@ -421,25 +434,26 @@ __global__ void beam_merge_kernel(const float* scores, const BeamPart* parts, co
   }
   __syncthreads();
   if (b != 0) return;
+  // what is picked is noted as beam << 8 | place and written out by all lanes afterwards: a step of the join is a chain that nothing hides
+  int* picked = reinterpret_cast<int*>(lists);
   BeamHead h(merged + lane * keep, lane < B ? keep : 0);
-  for (int n = 0; n < keep; ++n) {
+  int n = 0;
+  for (; n < keep; ++n) {
     const unsigned long long best = warp_max_key(h.head);
-    const size_t o = (size_t)g * keep + n;
-    if (best == 0) {
-      for (int i = n + lane; i < keep; i += 32) {
-        out_score[(size_t)g * keep + i] = -INFINITY;
-        out_parent[(size_t)g * keep + i] = -1;
-        out_token[(size_t)g * keep + i] = -1;
-      }
-      break;
-    }
-    const int who = __ffs(__ballot_sync(0xffffffffu, h.head == best)) - 1;     // of equal scores the first beam's
-    if (lane == who) {
-      out_score[o] = (float)double_of(best);
-      out_parent[o] = lane;
-      out_token[o] = best_token[lane * keep + h.at - 2];
+    if (best == 0) break;
+    const unsigned here = __ballot_sync(0xffffffffu, h.head == best);
+    if ((here & ((2u << lane) - 1)) == 1u << lane) {                           // of equal scores the first beam's
+      picked[n] = lane << 8 | (h.at - 2);
       h.pop();
     }
+  }
+  __syncwarp();
+  for (int i = lane; i < keep; i += 32) {
+    const size_t o = (size_t)g * keep + i;
+    const int which = i < n ? picked[i] : 0, from = (which >> 8) * keep + (which & 255);
+    out_score[o] = i < n ? (float)double_of(merged[from]) : -INFINITY;
+    out_parent[o] = i < n ? which >> 8 : -1;
+    out_token[o] = i < n ? best_token[from] : -1;
   }
 }
 
@@ -570,6 +584,16 @@ static int beam_log2_lanes(int keep) {             // four groups a wanted key, 
   return lg;
 }
 
+template <typename T>
+static bool beam_rows(const T* logits, int rows, int V, int keep, int splits, BeamPart* parts, unsigned long long* keys, cudaStream_t stream) {
+  static SharedLimit limit;
+  constexpr int N = BeamLoad<T>::N;
+  if (!limit.raise(beam_rows_kernel<T>, sizeof(BeamShared))) return false;
+  launch_kernel(beam_rows_kernel<T>, dim3((unsigned)(rows * splits)), BEAM_THREADS, sizeof(BeamShared), stream, logits, V, keep, beam_log2_lanes(keep), splits,
+                ((V + N - 1) / N + splits - 1) / splits, parts, keys);
+  return true;
+}
+
 }  // namespace sllm
 
 using namespace sllm;
@@ -586,23 +610,17 @@ SLLM_EXPORT int sllm_beam_candidates(const void* logits, int dtype, const float*
   SLLM_REQUIRE(dtype == SLLM_F32 || dtype == SLLM_BF16, "beam_candidates: unknown dtype %d", dtype);
   SLLM_REQUIRE(splits >= 1 && splits <= 32 && (long long)G * B * splits < (1ll << 31), "beam_candidates: %d parts a row", splits);
   if (G == 0) return SLLM_OK;
-  const int lanes = beam_log2_lanes(keep);
-  const int per = dtype == SLLM_F32 ? 4 : 8;
-  const int part_vecs = ((V + per - 1) / per + splits - 1) / splits;
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(scratch);
   BeamPart* parts = reinterpret_cast<BeamPart*>(keys + (size_t)G * B * splits * keep);
-  static SharedLimit limit_f, limit_b, limit_m;
+  static SharedLimit limit;
   const size_t merge_smem = beam_merge_smem(B, splits, keep);
-  if (!(dtype == SLLM_F32 ? limit_f.raise(beam_rows_kernel<float>, sizeof(BeamShared)) : limit_b.raise(beam_rows_kernel<__nv_bfloat16>, sizeof(BeamShared))) ||
-      !limit_m.raise(beam_merge_kernel, merge_smem)) {
+  bool there = limit.raise(beam_merge_kernel, merge_smem);
+  if (dtype == SLLM_F32) there = there && beam_rows((const float*)logits, G * B, V, keep, splits, parts, keys, stream);
+  else there = there && beam_rows((const __nv_bfloat16*)logits, G * B, V, keep, splits, parts, keys, stream);
+  if (!there) {
     set_error("beam_candidates: cannot raise the shared memory limit");
     return SLLM_ERR_LAUNCH;
   }
-  if (dtype == SLLM_F32)
-    launch_kernel(beam_rows_kernel<float>, dim3((unsigned)(G * B * splits)), BEAM_THREADS, sizeof(BeamShared), stream, (const float*)logits, V, keep, lanes, splits, part_vecs, parts, keys);
-  else
-    launch_kernel(beam_rows_kernel<__nv_bfloat16>, dim3((unsigned)(G * B * splits)), BEAM_THREADS, sizeof(BeamShared), stream, (const __nv_bfloat16*)logits, V, keep, lanes, splits, part_vecs, parts,
-                  keys);
   launch_kernel(beam_merge_kernel, G, 32 * B, merge_smem, stream, scores, (const BeamPart*)parts, (const unsigned long long*)keys, B, keep, splits, out_score, out_parent, out_token);
   return launch_status("beam_candidates");
 }
