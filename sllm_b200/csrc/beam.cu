@@ -91,9 +91,12 @@ template <> struct BeamLoad<__nv_bfloat16> {
 // a pass over a full list can leave.
 constexpr int BEAM_LIST = BEAM_KEEP * BEAM_VALUES + BEAM_KEEP, BEAM_OTHER = BEAM_LIST / 2 + BEAM_KEEP;
 
+constexpr int BEAM_SEEN = 256;                                  // threads' batches a warp can note in a run
+
 struct BeamShared {
   unsigned long long list[BEAM_LIST], other[BEAM_OTHER];
   unsigned long long group[BEAM_THREADS];
+  int seen[BEAM_THREADS / 32][BEAM_SEEN];
   unsigned long long bound;
   double red_s[BEAM_THREADS / 32];
   float red_m[BEAM_THREADS / 32];
@@ -185,10 +188,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 // together, the next batch's under the arithmetic of this one.
 // An exponential is 2^(x log2 e - c) in one rounding of the exponent: off by about |x - m| + 4 units of 2^-24, of which the sum keeps the mean, |x - m| being at most ln V on
 // average under the softmax itself.
-// Of a batch only keys that reach the bound, a key that `keep` others are known to reach, enter the list.  The first batch's bound comes from the threads' largest; then runs
-// of 3, 12, 48, ... batches are read without a barrier, every thread adding what reaches the bound, and the list, cut to its `keep` largest, gives the next bound: of logits in
-// no particular order three times `keep` a run.  Where a run finds more than the list holds (logits that rise through
-// the row), its batches are read again, one by one, each with a bound of its own.
+// Of a batch only keys that reach the bound, a key that `keep` others are known to reach, can be among the best.  The first batch's bound comes from the threads' largest.  A run of
+// 6, then 36, ... batches is read without a barrier; a thread whose largest logit of a batch reaches the bound notes the batch (a vote of its warp, no atomics), and behind the run the noted
+// ones are read again (from L1 or L2), their keys join the list, and the list, cut to its `keep` largest, gives the next bound: of logits in no particular order five or six
+// times `keep` a run.  Where a run has more than the lists hold (logits that rise through the row, or are equal), its batches are read again one by one, each with a bound of its own.
+// (512 rows of 152,064 bfloat16 logits, keep 16, us: reading them and their maxima 30, with the exponentials 37, with the list LIST_US; 50 where every thread put its keys
+// into the list at once.)
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_kernel(const T* logits, int V, int keep, int log2_lanes, int splits, int part_vecs, BeamPart* parts, unsigned long long* keys) {
   constexpr int N = BeamLoad<T>::N, LOADS = BEAM_VALUES / N, BATCH = LOADS * BEAM_THREADS;
@@ -205,17 +210,18 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
   unsigned long long bound = (unsigned long long)(BEAM_MINUS_INFINITY + 1) << 32;
   float bound_logit = beam_value(BEAM_MINUS_INFINITY + 1);
   float m = -INFINITY, s = 0.f;
-  auto fetch = [&](int vb, uint4* raw) {
-    if (vb + BATCH <= whole) {
-      const uint4* p = reinterpret_cast<const uint4*>(x_row) + vb + threadIdx.x;
+  // the pieces of one thread's batch: first, first + BEAM_THREADS, ...
+  auto fetch = [&](int first, bool all, uint4* raw) {
+    if (all) {
+      const uint4* p = reinterpret_cast<const uint4*>(x_row) + first;
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) raw[u] = p[u * BEAM_THREADS];
     } else {
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) {
-        const int v = vb + u * BEAM_THREADS + threadIdx.x, first = v * N;
-        if (v < whole) raw[u] = *reinterpret_cast<const uint4*>(x_row + first);
-        else raw[u] = BeamLoad<T>::gather(x_row + first, [&](int i) { return v < v1 && first + i < V; });
+        const int v = first + u * BEAM_THREADS, token = v * N;
+        if (v < whole) raw[u] = *reinterpret_cast<const uint4*>(x_row + token);
+        else raw[u] = BeamLoad<T>::gather(x_row + token, [&](int i) { return v < v1 && token + i < V; });
       }
     }
   };
@@ -266,16 +272,16 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     }
   };
   // a logit's key, 0 where it offers nothing; minus zero is zero
-  auto key_of = [&](float f, int vb, int i) {
+  auto key_of = [&](float f, int first, int i) {
     f += 0.0f;
-    return f > -INFINITY ? beam_key(f, (vb + (i / N) * BEAM_THREADS + (int)threadIdx.x) * N + i % N) : 0ull;
+    return f > -INFINITY ? beam_key(f, (first + (i / N) * BEAM_THREADS) * N + i % N) : 0ull;
   };
-  auto append = [&](const float* x, float top, int vb) {
+  auto append = [&](const float* x, float top, int first) {
     if (top >= bound_logit) {
 #pragma unroll
       for (int i = 0; i < BEAM_VALUES; ++i)
         if (x[i] >= bound_logit) {
-          const unsigned long long k = key_of(x[i], vb, i);
+          const unsigned long long k = key_of(x[i], first, i);
           if (k >= bound) {
             const int at = atomicAdd(&sh.n, 1);
             if (at < BEAM_LIST) sh.list[at] = k;
@@ -287,60 +293,69 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     bound = bound > b ? bound : b;
     bound_logit = beam_value((uint32_t)(bound >> 32));
   };
+  int held = 0;                                    // keys in the list behind a cut
   auto cut = [&]() {
-    if (beam_compact(keep, log2_lanes, sh) == keep) raise(sh.list[keep - 1]);
+    held = beam_compact(keep, log2_lanes, sh);
+    if (held == keep) raise(sh.list[keep - 1]);
     __syncthreads();
   };
-  // One batch behind a barrier: at most `keep` keys are in the list, and those of this batch from the keep-th largest of the groups' largest on join them, which are those of
-  // fewer than `keep` groups and one more.
-  auto add_batch = [&](const float* x, float top, int vb) {
+  // The bound of one batch: the keep-th largest of the groups' largest keys.  The keys that reach it are those of fewer than `keep` groups and one more.
+  auto bound_of = [&](const float* x, float top, int first) {
     int at = 0;
 #pragma unroll
-    for (int i = BEAM_VALUES - 1; i >= 0; --i) at = x[i] == top ? i : at;          // the first of the largest (of two zeros either will do: both reach the bound then)
-    raise(beam_group_bound(key_of(top, vb, at), log2_lanes, keep, sh));
-    append(x, top, vb);
+    for (int i = BEAM_VALUES - 1; i >= 0; --i) at = x[i] == top ? i : at;          // the first of the largest
+    raise(beam_group_bound(key_of(top, first, at), log2_lanes, keep, sh));
   };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4 next[LOADS];
   float x[BEAM_VALUES];
   __syncthreads();
   pdl_wait();
-  fetch(v0, next);
-  {
-    const float top = open(next, x);
-    if (v0 + BATCH < v1) fetch(v0 + BATCH, next);
-    add_up(x, top);
-    add_batch(x, top, v0);
-  }
-  int vb = v0 + BATCH;
-  for (int batches = 3; vb < v1; batches = min(4 * batches, 1 << 20)) {
-    __syncthreads();
-    const int held = sh.n, run = vb, end = min(vb + batches * BATCH, v1);
-    __syncthreads();
+  fetch(v0 + threadIdx.x, v0 + BATCH <= whole, next);
+  for (int vb = v0, batches = 6; vb < v1; batches = min(6 * batches, 1 << 20)) {
+    const int run = vb, end = min(vb + batches * BATCH, v1);
+    int noted = 0;
     for (; vb < end; vb += BATCH) {
       const float top = open(next, x);
-      if (vb + BATCH < v1) fetch(vb + BATCH, next);
+      if (vb + BATCH < v1) fetch(vb + BATCH + threadIdx.x, vb + 2 * BATCH <= whole, next);
       add_up(x, top);
-      append(x, top, vb);
+      if (vb == v0) bound_of(x, top, vb + threadIdx.x);
+      const unsigned votes = __ballot_sync(0xffffffffu, top >= bound_logit);
+      if (votes) {
+        const int at = noted + __popc(votes & ((1u << lane) - 1));
+        if (top >= bound_logit && at < BEAM_SEEN) sh.seen[warp][at] = vb + threadIdx.x;
+        noted += __popc(votes);
+      }
+    }
+    __syncwarp();
+    uint4 raw[LOADS];
+    if (noted <= BEAM_SEEN) {
+      for (int j = lane; j < noted; j += 32) {
+        const int first = sh.seen[warp][j];
+        fetch(first, false, raw);
+        const float top = open(raw, x);
+        append(x, top, first);
+      }
+    } else if (lane == 0) {
+      atomicAdd(&sh.n, BEAM_LIST + 1);
     }
     __syncthreads();
-    const int n = sh.n;
-    if (n > BEAM_LIST) {
+    if (sh.n <= BEAM_LIST) {
+      cut();
+    } else {
       __syncthreads();
       if (threadIdx.x == 0) sh.n = held;
-      cut();
-      uint4 raw[LOADS];
       for (int again = run; again < end; again += BATCH) {
-        fetch(again, raw);
-        add_batch(x, open(raw, x), again);
+        fetch(again + threadIdx.x, false, raw);
+        const float top = open(raw, x);
+        bound_of(x, top, again + threadIdx.x);     // (the list holds `keep` keys at most: it has room)
+        append(x, top, again + threadIdx.x);
         cut();
       }
-    } else if (n > keep) {
-      cut();
     }
   }
   pdl_launch_dependents();
   // the part's maximum and sum
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   s *= exp2_fast(-rest);
   const float wm = warp_max(m);
   double ws = (m > -INFINITY && (wm < INFINITY || m == wm)) ? (double)s * (m == wm ? 1.0 : exp((double)m - (double)wm)) : 0.0;
@@ -350,7 +365,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     sh.red_m[warp] = wm;
     sh.red_s[warp] = ws;
   }
-  const int n = beam_compact(keep, log2_lanes, sh);
+  __syncthreads();
   if (warp == 0) {
     const float wmax = lane < BEAM_THREADS / 32 ? sh.red_m[lane] : -INFINITY, all = warp_max(wmax);
     double sum = 0.0;
@@ -359,7 +374,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) parts[blockIdx.x] = BeamPart{sum, all};
   }
-  for (int i = threadIdx.x; i < keep; i += BEAM_THREADS) keys[(size_t)blockIdx.x * keep + i] = i < n ? sh.list[i] : 0ull;
+  for (int i = threadIdx.x; i < keep; i += BEAM_THREADS) keys[(size_t)blockIdx.x * keep + i] = i < held ? sh.list[i] : 0ull;
 }
 
 // A search: warp b joins the parts of beam b's row, then the first warp joins the beams.  Every step of a join takes the largest of the lists' heads, one a lane; the key behind a head
