@@ -192,8 +192,8 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 // 6, then 36, ... batches is read without a barrier; a thread whose largest logit of a batch reaches the bound notes the batch (a vote of its warp, no atomics), and behind the run the noted
 // ones are read again (from L1 or L2), their keys join the list, and the list, cut to its `keep` largest, gives the next bound: of logits in no particular order five or six
 // times `keep` a run.  Where a run has more than the lists hold (logits that rise through the row, or are equal), its batches are read again one by one, each with a bound of its own.
-// (512 rows of 152,064 bfloat16 logits, keep 16, us: reading them and their maxima 30, with the exponentials 37, with the list LIST_US; 50 where every thread put its keys
-// into the list at once.)
+// (512 rows of 152,064 bfloat16 logits, keep 16, us: reading them and their maxima 30, with the exponentials 37, with the list 48; 50 where every thread put its
+// keys into the list at once.)
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_kernel(const T* logits, int V, int keep, int log2_lanes, int splits, int part_vecs, BeamPart* parts, unsigned long long* keys) {
   constexpr int N = BeamLoad<T>::N, LOADS = BEAM_VALUES / N, BATCH = LOADS * BEAM_THREADS;
@@ -613,8 +613,18 @@ static bool beam_rows(const T* logits, int rows, int V, int keep, int splits, Be
 
 using namespace sllm;
 
-// parts a row is cut into, at most 32 (a lane of the merging warp each)
-SLLM_EXPORT int sllm_beam_splits(int G, int B, int V, int keep) { return 1; }
+// Parts a row is cut into: as many as the SMs hold blocks (four an SM) for all rows, none shorter than a batch, at most 32 (a lane of the merging warp each) and 64 lists a search, beyond which
+// the join costs what the parts save.  (us by parts, 152,064 float32 logits: 4 rows: 1 24, 8 11, 16 9.4, 32 9.2; 32 rows: 1 28, 4 19, 8 16, 16 16, 32 22; 128 rows: 1 39, 4 28, 8 31;
+// 256 rows: 1 45, 2 38, 4 46; 512 rows: 1 61, 2 67.)
+SLLM_EXPORT int sllm_beam_splits(int G, int B, int V) {
+  const long long rows = (long long)G * B;
+  long long n = rows > 0 ? 4ll * num_sms() / rows : 1;
+  const long long batches = (V + BEAM_VALUES * BEAM_THREADS - 1) / (BEAM_VALUES * BEAM_THREADS);
+  if (n > batches) n = batches;
+  if (n > 64 / B) n = 64 / B;
+  if (n > 32) n = 32;
+  return n < 1 ? 1 : (int)n;
+}
 
 // scratch: G * B * splits * (8 * keep + 16) bytes, every part's keys, then its sum and maximum
 SLLM_EXPORT int sllm_beam_candidates(const void* logits, int dtype, const float* scores, int G, int B, int V, int keep, int splits, void* scratch, float* out_score, int* out_parent,

@@ -33,46 +33,52 @@ struct ReorderPlan {
   long long unit;              // bytes a block copies at a time
 };
 
+constexpr int REORDER_LOADS = 4;                // a thread's copies in flight
+
+// `n` pieces of V, the block's threads side by side
 template <typename V>
-__device__ __forceinline__ void copy_run(unsigned char* dst, const unsigned char* src, long long n) {       // n: elements of V; the block's threads side by side, four in flight
+__device__ __forceinline__ void copy_run(unsigned char* dst, const unsigned char* src, int n) {
   V* d = reinterpret_cast<V*>(dst);
   const V* s = reinterpret_cast<const V*>(src);
-  for (long long i = threadIdx.x; i < n; i += 4 * REORDER_THREADS) {
-    V v[4];
+  for (int i = threadIdx.x; i < n; i += REORDER_LOADS * REORDER_THREADS) {
+    V v[REORDER_LOADS];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < REORDER_LOADS; ++u)
       if (i + u * REORDER_THREADS < n) v[u] = s[i + u * REORDER_THREADS];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < REORDER_LOADS; ++u)
       if (i + u * REORDER_THREADS < n) d[i + u * REORDER_THREADS] = v[u];
   }
 }
 
-// elements [from, to) of the written entries of a page: `per` elements of every head of every outer copy, one after the other
+// Pieces [from, from + n) of the written entries of a page: `per` pieces of every head of every outer copy, one after the other.
 template <typename V>
-__device__ __forceinline__ void copy_page(const PagedTable& t, int dst_page, int src_page, unsigned per, unsigned long long from, unsigned long long to) {
+__device__ __forceinline__ void copy_page(const PagedTable& t, int dst_page, int src_page, unsigned per, unsigned long long from, int n) {
   const size_t head_bytes = (size_t)t.page_size * t.entry_bytes, page_bytes = head_bytes * t.heads, outer_bytes = page_bytes * t.pages;
-  for (unsigned long long i0 = from + threadIdx.x; i0 < to; i0 += 4 * REORDER_THREADS) {
-    V v[4];
-    unsigned char* d[4];
+  // the unit's first segment once, then 32-bit steps from it
+  const unsigned seg0 = (unsigned)(from / per), at0 = (unsigned)(from - (unsigned long long)seg0 * per);
+  const long long move = ((long long)dst_page - src_page) * (long long)page_bytes;
+  unsigned char* base = t.base + (size_t)src_page * page_bytes;
+  for (int i0 = threadIdx.x; i0 < n; i0 += REORDER_LOADS * REORDER_THREADS) {
+    V v[REORDER_LOADS];
+    unsigned char* p[REORDER_LOADS];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const unsigned long long i = i0 + u * REORDER_THREADS;
-      d[u] = nullptr;
-      if (i < to) {
-        const unsigned seg = (unsigned)(i / per), at = (unsigned)(i - (unsigned long long)seg * per), o = seg / t.heads, h = seg - o * t.heads;
-        unsigned char* place = t.base + (size_t)o * outer_bytes + (size_t)h * head_bytes + (size_t)at * sizeof(V);
-        d[u] = place + (size_t)dst_page * page_bytes;
-        v[u] = *reinterpret_cast<const V*>(place + (size_t)src_page * page_bytes);
+    for (int u = 0; u < REORDER_LOADS; ++u) {
+      const int i = i0 + u * REORDER_THREADS;
+      p[u] = nullptr;
+      if (i < n) {
+        const unsigned k = at0 + (unsigned)i, seg = seg0 + k / per, at = k % per, o = seg / (unsigned)t.heads, h = seg % (unsigned)t.heads;
+        p[u] = base + (size_t)o * outer_bytes + (size_t)h * head_bytes + (size_t)at * sizeof(V);
+        v[u] = *reinterpret_cast<const V*>(p[u]);
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (d[u]) *reinterpret_cast<V*>(d[u]) = v[u];
+    for (int u = 0; u < REORDER_LOADS; ++u)
+      if (p[u]) *reinterpret_cast<V*>(p[u] + move) = v[u];
   }
 }
 
-__global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const int* parents, const int* slots, const int* lens, int* new_slots, int G, int B, const ReorderPlan plan) {
+__global__ void __launch_bounds__(REORDER_THREADS, 4) beam_reorder_kernel(const int* parents, const int* slots, const int* lens, int* new_slots, int G, int B, const ReorderPlan plan) {
   extern __shared__ int reorder_smem[];
   const int S = G * B;
   int* source = reorder_smem;                   // [S] the row a row goes on from
@@ -139,18 +145,9 @@ __global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const int
     if (threadIdx.x == REORDER_THREADS - 1) first_unit[S] = before;
   }
   __syncthreads();
-  // slots and tables
+  // slots
   if (new_slots != nullptr && blockIdx.x == 0)
     for (int r = threadIdx.x; r < S; r += REORDER_THREADS) new_slots[r] = slots[takes[r]];
-  for (int k = 0; k < plan.num_paged; ++k) {
-    const PagedTable& t = plan.paged[k];
-    for (int r = blockIdx.x; r < S; r += gridDim.x) {
-      const int entries = max(lens[r / B], 0) / t.stride, at = entries / t.page_size;
-      const bool begun = entries % t.page_size > 0;
-      const int *own = t.table + (size_t)r * t.columns, *from = t.table + (size_t)source[r] * t.columns, *taken = t.table + (size_t)takes[r] * t.columns;
-      for (int c = threadIdx.x; c < t.columns; c += REORDER_THREADS) t.new_table[(size_t)r * t.columns + c] = c < at ? from[c] : (c == at && begun) ? taken[c] : own[c];
-    }
-  }
   // the copies
   const int all = first_unit[S];
   for (int u = blockIdx.x; u < all; u += gridDim.x) {
@@ -172,7 +169,8 @@ __global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const int
           continue;
         }
         if (dst >= 0 && dst < t.slots && src >= 0 && src < t.slots) {
-          const long long b0 = at * plan.unit, bytes = min(plan.unit, t.row_bytes - b0);
+          const long long b0 = at * plan.unit;
+          const int bytes = (int)min(plan.unit, t.row_bytes - b0);
           unsigned char* d = t.base + (size_t)dst * t.row_bytes + b0;
           const unsigned char* s = t.base + (size_t)src * t.row_bytes + b0;
           if (t.width == 16) copy_run<uint4>(d, s, bytes / 16);
@@ -197,14 +195,25 @@ __global__ void __launch_bounds__(REORDER_THREADS) beam_reorder_kernel(const int
       if (column < t.columns) {
         const int src = t.table[(size_t)source[r] * t.columns + column], dst = t.table[(size_t)takes[r] * t.columns + column];
         if (src >= 0 && src < t.pages && dst >= 0 && dst < t.pages) {
-          const long long b0 = at * plan.unit, b1 = min(b0 + plan.unit, bytes);
+          const long long b0 = at * plan.unit;
+          const int n_bytes = (int)min(plan.unit, bytes - b0);
           const unsigned per = (unsigned)(written * t.entry_bytes / t.width);
-          if (t.width == 16) copy_page<uint4>(t, dst, src, per, b0 / 16, b1 / 16);
-          else if (t.width == 4) copy_page<uint32_t>(t, dst, src, per, b0 / 4, b1 / 4);
-          else copy_page<unsigned short>(t, dst, src, per, b0 / 2, b1 / 2);
+          if (t.width == 16) copy_page<uint4>(t, dst, src, per, b0 / 16, n_bytes / 16);
+          else if (t.width == 4) copy_page<uint32_t>(t, dst, src, per, b0 / 4, n_bytes / 4);
+          else copy_page<unsigned short>(t, dst, src, per, b0 / 2, n_bytes / 2);
         }
       }
       break;
+    }
+  }
+  // the tables: rows over the blocks
+  for (int k = 0; k < plan.num_paged; ++k) {
+    const PagedTable& t = plan.paged[k];
+    for (int r = blockIdx.x; r < S; r += gridDim.x) {
+      const int entries = max(lens[r / B], 0) / t.stride, at = entries / t.page_size;
+      const bool begun = entries % t.page_size > 0;
+      const int *own = t.table + (size_t)r * t.columns, *from = t.table + (size_t)source[r] * t.columns, *taken = t.table + (size_t)takes[r] * t.columns;
+      for (int c = threadIdx.x; c < t.columns; c += REORDER_THREADS) t.new_table[(size_t)r * t.columns + c] = c < at ? from[c] : (c == at && begun) ? taken[c] : own[c];
     }
   }
   pdl_launch_dependents();
@@ -333,8 +342,11 @@ SLLM_EXPORT int sllm_beam_reorder(const int* parents, const int* slots, const in
   ReorderPlan plan = {};
   plan.num_states = num_states;
   plan.num_paged = num_paged;
-  plan.unit = 16384;
-  long long units = 0, cells = 0;                // at most, a row
+  long long bytes = 0, units = 0, cells = 0;     // at most, a row
+  for (int k = 0; k < num_states; ++k) bytes += states[3 * k + 1];
+  for (int k = 0; k < num_paged; ++k) bytes += paged[10 * k + 3] * paged[10 * k + 4] * paged[10 * k + 5] * paged[10 * k + 7];
+  // A unit is a load a thread where that is what it takes to give every SM some (one page of 24 layers, 135 KB: UNIT_SMALL), else four.
+  plan.unit = bytes * G * B <= 16384ll * num_sms() ? REORDER_THREADS * 16 : REORDER_THREADS * 16 * REORDER_LOADS;
   for (int k = 0; k < num_states; ++k) {
     const long long* s = states + 3 * k;
     SLLM_REQUIRE(s[1] > 0 && s[1] < (1ll << 40) && s[2] > 0 && s[2] < (1ll << 31), "beam_reorder: state %d: %lld rows of %lld bytes", k, s[2], s[1]);
@@ -355,7 +367,7 @@ SLLM_EXPORT int sllm_beam_reorder(const int* parents, const int* slots, const in
     cells += p[9];
   }
   SLLM_REQUIRE(units * G * B < (1ll << 30), "beam_reorder: %lld bytes a beam", units * plan.unit);
-  const long long work = units * G * B + (cells * G * B + 1023) / 1024, most = (long long)num_sms() * 8;
+  const long long work = units * G * B + (cells * G * B + 1023) / 1024, most = (long long)num_sms() * 4;
   const int grid = (int)(work < 1 ? 1 : work < most ? work : most);
   launch_kernel(beam_reorder_kernel, grid, REORDER_THREADS, (size_t)(3 * G * B + 1) * sizeof(int), stream, parents, slots, lens, new_slots, G, B, plan);
   return launch_status("beam_reorder");

@@ -2625,6 +2625,7 @@ MAX_BEAMS, MAX_CANDIDATES, MAX_BEAM_ROWS = 32, 128, 2048
 
 BeamPool = namedtuple("BeamPool", "scores lengths parents tokens")
 BeamStep = namedtuple("BeamStep", "scores parents tokens lengths done pool")
+_NO_STEP = BeamStep(*(None,) * 5, BeamPool(*(None,) * 4))
 StepTables = namedtuple("StepTables", "q_start ctx_len positions seq_of_token block_tables slot_mappings")
 
 
@@ -2641,6 +2642,11 @@ def _typed(what: str, dtype, shape, *tensors) -> None:
     for t in tensors:
         if t.dtype is not dtype or t.shape != shape:
             raise KernelError(f"{what}: {t.dtype} {tuple(t.shape)}, not {dtype} {shape}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _beam_splits(device: int, G: int, B: int, V: int) -> int:
+    return lib().sllm_beam_splits(G, B, V)
 
 
 def beam_candidates(logits: torch.Tensor, scores: torch.Tensor, keep: int):
@@ -2663,7 +2669,7 @@ def beam_candidates(logits: torch.Tensor, scores: torch.Tensor, keep: int):
     tokens = torch.empty_like(parents)
     if G == 0:
         return out_s, parents, tokens
-    splits = lib().sllm_beam_splits(G, B, V, keep)
+    splits = _beam_splits(logits.get_device(), G, B, V)
     scratch = torch.empty(G * B * splits * (keep + 2), dtype=torch.int64, device=dev)
     call("sllm_beam_candidates", _p(logits), dt, _p(scores), G, B, V, keep, splits, _p(scratch), _p(out_s), _p(parents), _p(tokens), _stream())
     return out_s, parents, tokens
@@ -2690,8 +2696,10 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     0; a search that is over: minus infinity, each beam its own parent, 0), the new ``lengths``, ``done`` and ``pool``; a search that was over before keeps
     its pool and length.  ``out``: a `BeamStep` of tensors to write, the inputs' own among them.  At most 32 beams, a pool of 32 and 128 candidates."""
     if out is None:
-        out = BeamStep(*(None,) * 5, BeamPool(*(None,) * 4))
-    _here("beam_advance", scores, parents, tokens, *pool, lengths, done, stop_ids, *out[:5], *out.pool)
+        out = _NO_STEP
+        _here("beam_advance", scores, parents, tokens, *pool, lengths, done, stop_ids)
+    else:
+        _here("beam_advance", scores, parents, tokens, *pool, lengths, done, stop_ids, *out[:5], *out.pool)
     if scores.dim() != 2 or pool.scores.dim() != 2:
         raise KernelError("beam_advance: candidates [G, keep] and a pool [G, W]")
     (G, keep), W, beams, max_new, power = scores.shape, pool.scores.shape[1], int(beams), int(max_new), float(length_penalty)
@@ -2705,19 +2713,17 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     _typed("beam_advance: lengths and done", torch.int32, (G,), lengths, done)
     if stop_ids is not None and stop_ids.dtype != torch.int32:
         raise KernelError("beam_advance: stop ids are int32")
-    dev = scores.device
-
-    def place(t, what, dtype, shape, like):
-        if t is None:
-            return torch.empty(*shape, dtype=dtype, device=dev) if like is None else torch.empty_like(like)
-        _typed("beam_advance: out." + what, dtype, shape, t)
-        return t
-    i32, f32 = torch.int32, torch.float32
-    nxt_parents = place(out.parents, "parents", i32, (G, beams), None)
-    res = BeamStep(place(out.scores, "scores", f32, (G, beams), None), nxt_parents, place(out.tokens, "tokens", i32, (G, beams), nxt_parents),
-                   place(out.lengths, "lengths", i32, (G,), lengths), place(out.done, "done", i32, (G,), done),
-                   BeamPool(place(out.pool.scores, "pool.scores", f32, (G, W), pool.scores), place(out.pool.lengths, "pool.lengths", i32, (G, W), pool.lengths),
-                            place(out.pool.parents, "pool.parents", i32, (G, W), pool.parents), place(out.pool.tokens, "pool.tokens", i32, (G, W), pool.tokens)))
+    i32, f32, dev = torch.int32, torch.float32, scores.device
+    new = torch.empty(G, beams, dtype=i32, device=dev) if out.parents is None else out.parents
+    res = BeamStep(torch.empty(G, beams, dtype=f32, device=dev) if out.scores is None else out.scores, new, torch.empty_like(new) if out.tokens is None else out.tokens,
+                   torch.empty_like(lengths) if out.lengths is None else out.lengths, torch.empty_like(done) if out.done is None else out.done,
+                   BeamPool(*[torch.empty_like(a) if b is None else b for a, b in zip(pool, out.pool)]))
+    if out is not _NO_STEP:
+        _typed("beam_advance: out.scores", f32, (G, beams), res.scores)
+        _typed("beam_advance: out.parents and tokens", i32, (G, beams), res.parents, res.tokens)
+        _typed("beam_advance: out.lengths and done", i32, (G,), res.lengths, res.done)
+        _typed("beam_advance: out.pool", f32, (G, W), res.pool.scores)
+        _typed("beam_advance: out.pool", i32, (G, W), *res.pool[1:])
     if G:
         call("sllm_beam_advance", _p(scores), _p(parents), _p(tokens), G, keep, beams, W, *(_p(t) for t in pool), _p(lengths), _p(done),
              _p(stop_ids), stop_ids.numel() if stop_ids is not None else 0, max_new, ctypes.byref(ctypes.c_double(power)),

@@ -207,7 +207,7 @@ def _declare(L):
                                      c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
         "sllm_gated_group_norm": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_int, c_int, c_int,
                                   c_void_p],
-        "sllm_beam_splits": [c_int, c_int, c_int, c_int],
+        "sllm_beam_splits": [c_int, c_int, c_int],
         "sllm_beam_candidates": [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
         "sllm_beam_advance": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                               c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
