@@ -37,7 +37,9 @@ class RequestCache:
     req_id: object
     slot: int
     num_tokens: int = 0                       # tokens committed to the cache
-    tables: list[list[int]] = field(default_factory=list)   # per group: page ids, -1 once released
+    tables: list[list[int]] = field(default_factory=list)   # per group: page ids, -1 once released (or another request's: `fork_request`)
+    forked_from: object = None                # the request whose whole pages this one reads
+    forks: int = 0                            # live requests that read this one's
 
 
 class CacheManager:
@@ -236,10 +238,37 @@ class CacheManager:
                 for i in range(min(first, len(table))):
                     table[i] = -1
 
+    def fork_pages(self, req_id, total_tokens: int) -> list[int]:
+        """Per group: the pages a fork of the request takes to hold ``total_tokens``."""
+        n = self.requests[req_id].num_tokens
+        return [max(0, self.pages_for(total_tokens, gi) - n // g.need.stride // self.page_size) for gi, g in enumerate(self.groups)]
+
+    def fork_request(self, req_id, new_id, total_tokens: int) -> RequestCache:
+        """A request that goes on from ``req_id``'s tokens: the pages these fill are read by both and stay ``req_id``'s (-1 in the
+        new request's table), which has to outlive its forks; from the first page that is not full on it has pages of its own, up to ``total_tokens``, and a
+        state slot.  What lies in ``req_id``'s last page and slot is the caller's to copy (`ops.beam_reorder`).  Takes everything or nothing."""
+        src = self.requests[req_id]
+        if src.forked_from is not None:
+            raise ValueError(f"request {req_id!r} is a fork itself")
+        if total_tokens < src.num_tokens:
+            raise ValueError(f"request {req_id!r} holds {src.num_tokens} tokens, a fork of it cannot hold {total_tokens}")
+        for gi, (need, g) in enumerate(zip(self.fork_pages(req_id, total_tokens), self.groups)):
+            if need > g.pool.free_count:
+                raise OutOfPages(f"a fork of request {req_id!r} needs {need} pages in group {gi}, {g.pool.free_count} free of {g.pool.capacity}")
+        req = self.add_request(new_id)
+        req.num_tokens = src.num_tokens
+        req.tables = [[-1] * (src.num_tokens // g.need.stride // self.page_size) for g in self.groups]
+        req.forked_from = req_id
+        src.forks += 1
+        self.reserve(new_id, total_tokens)
+        return req
+
     def free_request(self, req_id) -> None:
         req = self.requests.get(req_id)
         if req is None:
             raise KeyError(f"request {req_id!r} is not live")
+        if req.forks:
+            raise ValueError(f"request {req_id!r}: {req.forks} forks still read its pages")
         # free before forgetting: an ownership error must not lose the table
         for gi, g in enumerate(self.groups):
             held = [p for p in req.tables[gi] if p >= 0]
@@ -247,6 +276,8 @@ class CacheManager:
             if self.poison_freed:
                 self._fill_pages(gi, held, float("nan"))
         self.slots.free(req_id, req.slot)
+        if req.forked_from is not None:
+            self.requests[req.forked_from].forks -= 1
         del self.requests[req_id]
 
     def _fill_pages(self, group: int, pages, value: float) -> None:

@@ -78,7 +78,7 @@ __device__ __forceinline__ void copy_page(const PagedTable& t, int dst_page, int
   }
 }
 
-__global__ void __launch_bounds__(REORDER_THREADS, 4) beam_reorder_kernel(const int* parents, const int* slots, const int* lens, int* new_slots, int G, int B, const ReorderPlan plan) {
+__global__ void __launch_bounds__(REORDER_THREADS, 4) beam_reorder_kernel(const int* parents, const int* slots, const int* lens, int len_step, int* new_slots, int G, int B, const ReorderPlan plan) {
   extern __shared__ int reorder_smem[];
   const int S = G * B;
   int* source = reorder_smem;                   // [S] the row a row goes on from
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(REORDER_THREADS, 4) beam_reorder_kernel(const 
         units = state_units;
         for (int k = 0; k < plan.num_paged; ++k) {
           const PagedTable& t = plan.paged[k];
-          const long long written = max(lens[g], 0) / t.stride % t.page_size;
+          const long long written = max(lens[g * len_step], 0) / t.stride % t.page_size;
           if (written > 0) units += (int)((written * t.entry_bytes * t.heads * t.outer + plan.unit - 1) / plan.unit);
         }
       }
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(REORDER_THREADS, 4) beam_reorder_kernel(const 
     at -= state_units;
     for (int k = 0; k < plan.num_paged; ++k) {
       const PagedTable& t = plan.paged[k];
-      const int entries = max(lens[r / B], 0) / t.stride, written = entries % t.page_size, column = entries / t.page_size;
+      const int entries = max(lens[r / B * len_step], 0) / t.stride, written = entries % t.page_size, column = entries / t.page_size;
       if (written == 0) continue;
       const long long bytes = (long long)written * t.entry_bytes * t.heads * t.outer;
       const int n = (int)((bytes + plan.unit - 1) / plan.unit);
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(REORDER_THREADS, 4) beam_reorder_kernel(const 
   for (int k = 0; k < plan.num_paged; ++k) {
     const PagedTable& t = plan.paged[k];
     for (int r = blockIdx.x; r < S; r += gridDim.x) {
-      const int entries = max(lens[r / B], 0) / t.stride, at = entries / t.page_size;
+      const int entries = max(lens[r / B * len_step], 0) / t.stride, at = entries / t.page_size;
       const bool begun = entries % t.page_size > 0;
       const int *own = t.table + (size_t)r * t.columns, *from = t.table + (size_t)source[r] * t.columns, *taken = t.table + (size_t)takes[r] * t.columns;
       for (int c = threadIdx.x; c < t.columns; c += REORDER_THREADS) t.new_table[(size_t)r * t.columns + c] = c < at ? from[c] : (c == at && begun) ? taken[c] : own[c];
@@ -333,8 +333,8 @@ __global__ void __launch_bounds__(TABLES_THREADS) step_tables_kernel(const int* 
 using namespace sllm;
 
 // `states` (on the host): base, bytes a row, rows of each table; `paged` (on the host), 10 numbers each: base, table, new table, bytes of an entry of one head, outer, heads, pages,
-// page size, stride, columns.  new_slots may be null.
-SLLM_EXPORT int sllm_beam_reorder(const int* parents, const int* slots, const int* lens, int* new_slots, int G, int B, const long long* states, int num_states,
+// page size, stride, columns.  lens[g * len_step] tokens are in search g's caches.  new_slots may be null.
+SLLM_EXPORT int sllm_beam_reorder(const int* parents, const int* slots, const int* lens, int len_step, int* new_slots, int G, int B, const long long* states, int num_states,
                                   const long long* paged, int num_paged, cudaStream_t stream) {
   SLLM_REQUIRE(G >= 0 && B >= 1 && B <= 32 && (long long)G * B <= REORDER_ROWS, "beam_reorder: %d searches of %d beams (at most 32, %d in all)", G, B, REORDER_ROWS);
   SLLM_REQUIRE(num_states >= 0 && num_states <= REORDER_STATES && num_paged >= 0 && num_paged <= REORDER_PAGED, "beam_reorder: %d states, %d paged caches", num_states, num_paged);
@@ -369,7 +369,7 @@ SLLM_EXPORT int sllm_beam_reorder(const int* parents, const int* slots, const in
   SLLM_REQUIRE(units * G * B < (1ll << 30), "beam_reorder: %lld bytes a beam", units * plan.unit);
   const long long work = units * G * B + (cells * G * B + 1023) / 1024, most = (long long)num_sms() * 4;
   const int grid = (int)(work < 1 ? 1 : work < most ? work : most);
-  launch_kernel(beam_reorder_kernel, grid, REORDER_THREADS, (size_t)(3 * G * B + 1) * sizeof(int), stream, parents, slots, lens, new_slots, G, B, plan);
+  launch_kernel(beam_reorder_kernel, grid, REORDER_THREADS, (size_t)(3 * G * B + 1) * sizeof(int), stream, parents, slots, lens, len_step, new_slots, G, B, plan);
   return launch_status("beam_reorder");
 }
 

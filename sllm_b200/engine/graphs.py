@@ -114,6 +114,27 @@ class Launched:
         self.graph, self.turn, self.ids_now, self.n = graph, turn, ids_now, n
 
 
+def captured(run, launches: int):
+    """``run()``'s launches (``launches`` of this package's kernels) as a graph, and how many of them report through the status word."""
+    graph = torch.cuda.CUDAGraph()
+    # Nothing may free device memory or destroy a graph while the capture runs: a collection
+    # of garbage (an engine dropped earlier, say) in the middle of it would invalidate it.
+    # (torch's graph context collects once before it begins; here the collector stays off.)
+    gc_was_on = gc.isenabled()
+    gc.disable()
+    reporting = ops.status_word_launches()
+    try:
+        with torch.cuda.graph(graph):
+            run()
+    finally:
+        if gc_was_on:
+            gc.enable()
+    ops.launches["own"] -= launches             # capturing launched nothing
+    reporting = ops.status_word_launches() - reporting      # kernels of the graph that report through the status word
+    ops.note_status_word_launches(-reporting)
+    return graph, reporting
+
+
 class DecodeGraphs:
     def __init__(self, engine):
         self.engine = engine
@@ -160,28 +181,11 @@ class DecodeGraphs:
     def _capture(self, gr: _Graph) -> torch.Tensor:
         """Run the step that `gr`'s static buffers describe once, launch by launch, then capture the same
         launches as a graph.  Returns the ids the eager run sampled."""
-        eng = self.engine
         before = ops.launches["own"]
-        gr.run(eng)
+        gr.run(self.engine)
         gr.launches = ops.launches["own"] - before
         eager_ids = gr.ids
-        graph = torch.cuda.CUDAGraph()
-        # Nothing may free device memory or destroy a graph while the capture runs: a collection
-        # of garbage (an engine dropped earlier, say) in the middle of it would invalidate it.
-        # (torch's graph context collects once before it begins; here the collector stays off.)
-        gc_was_on = gc.isenabled()
-        gc.disable()
-        reporting = ops.status_word_launches()
-        try:
-            with torch.cuda.graph(graph):
-                gr.run(eng)
-        finally:
-            if gc_was_on:
-                gc.enable()
-        ops.launches["own"] -= gr.launches          # capturing launched nothing
-        gr.reporting = ops.status_word_launches() - reporting      # kernels of the graph that report through the status word
-        ops.note_status_word_launches(-gr.reporting)
-        gr.graph = graph
+        gr.graph, gr.reporting = captured(lambda: gr.run(self.engine), gr.launches)
         return eager_ids
 
     def warmup(self, batch_sizes, contexts, penalised: bool = False) -> int:

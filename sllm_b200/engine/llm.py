@@ -18,7 +18,8 @@ from dataclasses import dataclass
 import torch
 
 from .. import ops
-from ..sampling import Sampler, SamplingParams
+from ..sampling import BeamParams, Sampler, SamplingParams
+from .beam import BeamSearch
 from .engine import Engine, StepEntry
 from .loading import build_model, parse_dtype
 from .scheduler import Scheduler
@@ -80,6 +81,7 @@ class LLM:
         self.cuda_graphs = bool(cuda_graphs) and model.device.type == "cuda"
         self.pipeline_decode = self.cuda_graphs and bool(pipeline_decode)
         self._inflight = None
+        self._beams = None
         self._next_id = 0
         self.steps = 0
 
@@ -218,3 +220,11 @@ class LLM:
         if not self.scheduler.has_work:
             self.drain()
         return [GenerationResult(r.req_id, r.prompt, list(r.output), r.finish_reason, r.preemptions) for r in reqs]
+
+    def beam_search(self, prompt_token_ids, params: BeamParams | None = None) -> list:
+        """Search for each prompt (a list of token ids): its `BeamResult`s, best first, in the prompts' order.  A search holds ``params.beams`` of the
+        ``max_num_seqs`` state slots; as many prompts as fit into the free slots and pages run side by side.  Requests that the scheduler is running keep what they hold and
+        wait meanwhile."""
+        if self._beams is None:
+            self._beams = BeamSearch(self.engine, chunk_size=self.scheduler.chunk_size, max_batch_tokens=self.scheduler.max_batch_tokens, cuda_graphs=self.cuda_graphs)
+        return self._beams.search(prompt_token_ids, params)

@@ -2629,13 +2629,17 @@ _NO_STEP = BeamStep(*(None,) * 5, BeamPool(*(None,) * 4))
 StepTables = namedtuple("StepTables", "q_start ctx_len positions seq_of_token block_tables slot_mappings")
 
 
-def _here(what: str, *tensors) -> None:
+def _here(what: str, first, *tensors) -> None:
     """`_chk`, and all on the current device: the launch goes to its current stream."""
-    index = _current_device() if _current_device is not None else torch.cuda.current_device()
+    index = first.get_device()
+    _chk(first)
     for t in tensors:
         if t is not None and (t.get_device() != index or not t.is_contiguous()):
             _chk(t)
-            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{index}")
+            raise KernelError(f"{what}: tensors on {t.device} and {first.device}")
+    now = _current_device() if _current_device is not None else torch.cuda.current_device()
+    if index != now:
+        raise KernelError(f"{what}: tensors on {first.device}, the current device is cuda:{now}")
 
 
 def _typed(what: str, dtype, shape, *tensors) -> None:
@@ -2736,7 +2740,7 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
 
     ``slots`` (int32 ``[G*B]``) names each beam's row in every tensor of ``states`` (``[rows, ...]``, any type); ``paged`` lists
     ``(storage [..., pages, heads, page size, head size], block table int32 [G*B, columns], stride)``, caches that hold an entry per ``stride`` tokens; ``lens``
-    (int32 ``[G]``) tokens are in a search's caches.  A parent's first child keeps its slot and its page that is only partly written; the other children get copies
+    (int32 ``[G]``, or ``[G*B]`` with equal numbers within a search) tokens are in a search's caches.  A parent's first child keeps its slot and its page that is only partly written; the other children get copies
     of the row and of the page's entries, in the slots and pages of beams without a child, in order; pages before that one are shared, those behind it stay each
     beam's own.  A beam with parent -1 takes such a place as it is.  Each slot, and each page from the first that is partly written on, belongs to one beam.
 
@@ -2751,7 +2755,7 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
         raise KernelError(f"beam_reorder: {G} searches of {B} beams (at most {MAX_BEAMS}, {MAX_BEAM_ROWS} in all)")
     _typed("beam_reorder: parents", torch.int32, (G, B), parents)
     _typed("beam_reorder: slots", torch.int32, (G * B,), slots)
-    _typed("beam_reorder: lens", torch.int32, (G,), lens)
+    _typed("beam_reorder: lens", torch.int32, (G * B,) if lens.numel() != G else (G,), lens)
     if new_slots is None:
         new_slots = torch.empty_like(slots)
     _typed("beam_reorder: new slots", torch.int32, (G * B,), new_slots)
@@ -2787,7 +2791,7 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
     while first or rows or about:             # (64 states and 8 caches a launch)
         s, p = rows[:3 * 64], about[:10 * 8]
         rows, about = rows[3 * 64:], about[10 * 8:]
-        call("sllm_beam_reorder", _p(parents), _p(slots), _p(lens), _p(new_slots) if first else None, G, B, (ctypes.c_longlong * len(s))(*s), len(s) // 3,
+        call("sllm_beam_reorder", _p(parents), _p(slots), _p(lens), lens.numel() // G, _p(new_slots) if first else None, G, B, (ctypes.c_longlong * len(s))(*s), len(s) // 3,
              (ctypes.c_longlong * len(p))(*p), len(p) // 10, _stream())
         first = False
     return new_slots, made

@@ -1,4 +1,4 @@
-from .params import SamplingParams
+from .params import BeamParams, SamplingParams
 from .sampler import Sampler
 
-__all__ = ["SamplingParams", "Sampler"]
+__all__ = ["BeamParams", "SamplingParams", "Sampler"]

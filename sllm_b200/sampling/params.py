@@ -33,3 +33,34 @@ class SamplingParams:
         """Whether a repetition penalty applies (runtime/sampler.py:24: none, <= 0 and 1 change nothing)."""
         p = self.repetition_penalty
         return p is not None and p > 0 and p != 1.0
+
+
+@dataclass
+class BeamParams:
+    """What a request asks of a beam search (the reference has none).  ``beams`` continuations are kept alive; a continuation ends with a token of
+    ``stop_ids`` (not part of its output) or at ``max_new`` tokens; finished ones are ranked by cumulative log-probability over
+    ``n ** length_penalty``, n their tokens with the stop; the ``results`` best come back (None: as many as beams).  The search ends when no living continuation could
+    still get among them, so that its results are those of a search to the last token."""
+    beams: int = 4
+    max_new: int = 16
+    length_penalty: float = 1.0
+    stop_ids: tuple = ()
+    results: int | None = None
+
+    def __post_init__(self):
+        self.stop_ids = tuple(sorted({int(s) for s in self.stop_ids}))
+        if self.results is None:
+            self.results = self.beams
+        if not 1 <= self.beams <= 32 or not 1 <= self.results <= 32:
+            raise ValueError("beams and results are 1 to 32")
+        if self.max_new < 1:
+            raise ValueError("max_new must be >= 1")
+        if not abs(self.length_penalty) < 64:
+            raise ValueError("length_penalty must be between -64 and 64")
+        if self.keep > 128:
+            raise ValueError(f"{self.beams} beams with {len(self.stop_ids)} stop ids need {self.keep} candidates a step, 128 at most")
+
+    @property
+    def keep(self) -> int:
+        """Candidates a step: every beam may lose one to each stop id, and as many as there are beams have to go on."""
+        return self.beams * (1 + len(self.stop_ids))

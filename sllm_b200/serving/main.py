@@ -9,7 +9,7 @@ and its dev command line (serving/cli.py:18-23: ``--temperature``, ``--top-p``,
 (serving/main.py:250-259).  ``serve`` (the HTTP server), ``--cpu`` and
 ``--placement um`` (host-memory decode) name things this engine does not have and
 are refused with a plain sentence.  Added here: ``--prompt-ids``, ``--dtype``,
-``--random-weights SEED``.
+``--random-weights SEED``, ``--beams`` and ``--length-penalty`` (a beam search in sampling's place).
 """
 
 from __future__ import annotations
@@ -97,6 +97,8 @@ def main(argv=None) -> int:
     ap.add_argument("--top-k", type=int, default=None)
     ap.add_argument("--seed", type=int, default=None)
     ap.add_argument("--repetition-penalty", type=float, default=None)
+    ap.add_argument("--beams", type=int, default=None, metavar="N", help="beam search with N beams; the best continuation is printed")
+    ap.add_argument("--length-penalty", type=float, default=1.0, help="of a beam search: scores are over tokens ** this")
     ap.add_argument("--dtype", choices=("bfloat16", "float32", "bf16", "fp32"), default=None)
     ap.add_argument("--random-weights", type=int, default=None, metavar="SEED",
                     help="write a random model folder from the recipe's geometry and run it")
@@ -115,6 +117,8 @@ def main(argv=None) -> int:
         ap.error("the following arguments are required: recipe")
     if args.cpu or args.placement == "um":
         raise SystemExit("sllm: this engine has no CPU or host-memory path; it runs on one B200")
+    if args.beams is not None and (args.temperature > 0 or args.top_k is not None or args.top_p is not None or args.repetition_penalty is not None):
+        raise SystemExit("sllm: --beams searches; it takes no --temperature, --top-k, --top-p or --repetition-penalty")
     if args.nodes not in (None, 1):
         raise SystemExit(f"sllm: --tp {args.nodes}: this engine runs on one GPU")
     try:
@@ -126,7 +130,7 @@ def main(argv=None) -> int:
     settings = {
         "dtype": dtype,
         "max_new": args.max_new if args.max_new is not None else int(de.get("max_new", 32)),
-        "max_num_seqs": int(de.get("max_num_seqs", 8)), "block_size": int(de.get("block_size", 16)),
+        "max_num_seqs": max(int(de.get("max_num_seqs", 8)), args.beams or 0), "block_size": int(de.get("block_size", 16)),
         "chunk_size": int(de.get("chunk_size", 512)), "max_model_len": de.get("max_model_len"),
     }
     model_dir = args.model_dir or recipe.local_dir
@@ -148,7 +152,11 @@ def main(argv=None) -> int:
         if not model_dir or not os.path.isdir(model_dir):
             raise SystemExit(f"sllm: weights not found: {model_dir or '(no path)'}")     # serving/main.py:239-240
         from ..engine.llm import LLM
-        from ..sampling import SamplingParams
+        from ..sampling import BeamParams, SamplingParams
+        try:
+            beams = BeamParams(beams=args.beams, max_new=settings["max_new"], length_penalty=args.length_penalty) if args.beams is not None else None
+        except ValueError as e:
+            raise SystemExit(f"sllm: {e}") from None
         llm = LLM(model_dir, dtype=dtype, block_size=settings["block_size"], max_num_seqs=settings["max_num_seqs"],
                   chunk_size=settings["chunk_size"], max_model_len=settings["max_model_len"],
                   kv_utilization=recipe.kv_utilization, kv_bytes=recipe.kv_device_bytes,
@@ -167,7 +175,14 @@ def main(argv=None) -> int:
                                 top_p=args.top_p, seed=args.seed, repetition_penalty=args.repetition_penalty)
         import time
         t0 = time.perf_counter()
-        results = llm.generate(prompts, params)
+        if beams is not None:
+            found = llm.beam_search(prompts, beams)
+            for i, f in enumerate(found):
+                for r in f:
+                    log("INFO", f"prompt {i}: {r.score:.4f} {r.finish_reason} {','.join(map(str, r.ids))}")
+            results = [f[0] for f in found]
+        else:
+            results = llm.generate(prompts, params)
         dt = time.perf_counter() - t0
         n_out = sum(len(r.ids) for r in results)
         log("INFO", f"prompt={sum(len(p) for p in prompts)} out={n_out} wall={dt:.3f}s ({n_out / max(dt, 1e-9):.1f} tok/s) "

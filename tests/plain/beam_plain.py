@@ -228,7 +228,7 @@ def beam_advance(scores, parents, tokens, pool, lengths, done, *, beams, stop_id
 
 def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
     paged = [(s.numpy() if s.dtype != torch.bfloat16 else s.view(torch.int16).numpy(), t.numpy(), st) for s, t, st in paged]
-    new_slots, tables = reorder(parents.numpy(), slots.numpy(), lens.numpy(), [s.numpy() for s in states], paged)
+    new_slots, tables = reorder(parents.numpy(), slots.numpy(), lens.numpy()[::max(1, lens.numel() // max(1, parents.shape[0]))], [s.numpy() for s in states], paged)
     o = out if out is not None else (None, [None] * len(tables))
     return _put(o[0], _i32(new_slots)), [_put(a, _i32(b)) for a, b in zip(o[1], tables)]
 
