@@ -114,12 +114,14 @@ __device__ unsigned long long beam_group_bound(unsigned long long mine, int log2
   if ((threadIdx.x & ((1 << log2_lanes) - 1)) == 0) sh.group[threadIdx.x >> log2_lanes] = mine;
   if (threadIdx.x == 0) sh.bound = 0;
   __syncthreads();
-  if (threadIdx.x < groups) {
-    const unsigned long long me = sh.group[threadIdx.x];
+  // a group's threads share the comparisons of its rank
+  {
+    const int lanes = 1 << log2_lanes, mine_at = threadIdx.x >> log2_lanes;
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < groups; ++j) rank += sh.group[j] > me || (sh.group[j] == me && j < (int)threadIdx.x);
-    if (rank == keep - 1) sh.bound = me;
+#pragma unroll 4
+    for (int j = threadIdx.x & (lanes - 1); j < groups; j += lanes) rank += sh.group[j] > mine || (sh.group[j] == mine && j < mine_at);
+    for (int o = 1; o < lanes; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (rank == keep - 1) sh.bound = mine;
   }
   __syncthreads();
   const unsigned long long b = sh.bound;
@@ -355,24 +357,20 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     }
   }
   pdl_launch_dependents();
-  // the part's maximum and sum
-  s *= exp2_fast(-rest);
-  const float wm = warp_max(m);
-  double ws = (m > -INFINITY && (wm < INFINITY || m == wm)) ? (double)s * (m == wm ? 1.0 : exp((double)m - (double)wm)) : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
-  if (lane == 0) {
-    sh.red_m[warp] = wm;
-    sh.red_s[warp] = ws;
-  }
+  // the part's maximum and sum: the threads' sums, brought to the same maximum, in 64 bits
+  const float warp_top = warp_max(m);
+  if (lane == 0) sh.red_m[warp] = warp_top;
   __syncthreads();
-  if (warp == 0) {
-    const float wmax = lane < BEAM_THREADS / 32 ? sh.red_m[lane] : -INFINITY, all = warp_max(wmax);
-    double sum = 0.0;
-    if (wmax > -INFINITY && (all < INFINITY || wmax == all)) sum = sh.red_s[lane] * (wmax == all ? 1.0 : exp((double)wmax - (double)all));
+  const float all = warp_max(lane < BEAM_THREADS / 32 ? sh.red_m[lane] : -INFINITY);
+  double sum = m == all && m > -INFINITY ? (double)(s * exp2_fast(-rest)) : m > -INFINITY && all < INFINITY ? (double)(s * exp2_fast((m - all) * log2e - rest)) : 0.0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) parts[blockIdx.x] = BeamPart{sum, all};
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sh.red_s[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < BEAM_THREADS / 32; ++w) sum += sh.red_s[w];
+    parts[blockIdx.x] = BeamPart{sum, all};
   }
   for (int i = threadIdx.x; i < keep; i += BEAM_THREADS) keys[(size_t)blockIdx.x * keep + i] = i < held ? sh.list[i] : 0ull;
 }
@@ -614,7 +612,7 @@ static bool beam_rows(const T* logits, int rows, int V, int keep, int splits, Be
 using namespace sllm;
 
 // Parts a row is cut into: as many as the SMs hold blocks (four an SM) for all rows, none shorter than a batch, at most 32 (a lane of the merging warp each) and 64 lists a search, beyond which
-// the join costs what the parts save.  (us by parts, 152,064 float32 logits: 4 rows: 1 24, 8 11, 16 9.4, 32 9.2; 32 rows: 1 28, 4 19, 8 16, 16 16, 32 22; 128 rows: 1 39, 4 28, 8 31;
+// the join costs what the parts save.  (us by parts, 152,064 float32 logits: 4 rows: 1 23, 8 11, 16 9.4, 32 8.7; 32 rows: 1 27, 4 18, 8 15, 16 16, 32 21; 128 rows: 1 39, 4 28, 8 30;
 // 256 rows: 1 45, 2 38, 4 46; 512 rows: 1 61, 2 67.)
 SLLM_EXPORT int sllm_beam_splits(int G, int B, int V) {
   const long long rows = (long long)G * B;

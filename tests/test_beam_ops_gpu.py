@@ -12,9 +12,10 @@ from tests.plain import beam_plain as plain
 
 pytestmark = pytest.mark.gpu
 
-# A score s + (d - log sum) off by: the rounding of the result (2^-24 of it), and the relative error of the sum of exponentials, which an exponential of a rounded difference
-# |d| <= 32 can have (2^-24 * 32 for the difference, 2 units for expf, 2^-24 * 40 for a thread's up to 600 terms in pairs of partial sums).
-SCORE = lambda s: 2.0 ** -24 * np.abs(s) + 2.0 ** -24 * (32 + 2 + 40)      # noqa: E731
+# A score s + (d - log sum) is off by the rounding of the result, 2^-24 of it, and by the relative error of the sum of exponentials, in units of 2^-24, which are means under the softmax
+# itself, where |x - max| is ln V <= 12 at the most: a thread's exponentials 19 (one rounding of the exponent 12, log2 e's own 3, the hardware's 2^-22 4), its sum 27 (8 additions
+# of a batch and up to 19 batches of these rows' parts), the threads' sums brought to one maximum 28 (a difference and a product 12 each, 4): 74.  What follows is 64 bits.
+SCORE = lambda s: 2.0 ** -24 * np.abs(s) + 2.0 ** -24 * (19 + 27 + 28)      # noqa: E731
 
 
 def _i32(a, dev):
