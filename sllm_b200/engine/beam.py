@@ -14,7 +14,7 @@ when they are.
 from __future__ import annotations
 
 from collections import OrderedDict
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 import torch
@@ -138,7 +138,7 @@ class BeamSearch:
 
     def search(self, prompts, params: BeamParams | None = None) -> list:
         """Per prompt (a list of token ids), its `BeamResult`s, best first.  Prompts that fit side by side run side by side."""
-        params = params or BeamParams()
+        params = replace(params or BeamParams())         # (checked again, and ours: the kept graphs are made for it)
         prompts = [[int(t) for t in p] for p in prompts]
         eng = self.engine
         for p in prompts:

@@ -2710,14 +2710,15 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     if not 1 <= keep <= MAX_CANDIDATES or not 1 <= beams <= MAX_BEAMS or not 1 <= W <= MAX_BEAMS or not 1 <= max_new < 1 << 30 or not abs(power) < 64:
         raise KernelError(f"beam_advance: {keep} candidates (1 to {MAX_CANDIDATES}), {beams} beams and a pool of {W} (1 to {MAX_BEAMS}), "
                           f"max_new {max_new}, length penalty {power}")
-    _typed("beam_advance: scores", torch.float32, (G, keep), scores)
-    _typed("beam_advance: parents and tokens", torch.int32, (G, keep), parents, tokens)
-    _typed("beam_advance: the pool's scores", torch.float32, (G, W), pool.scores)
-    _typed("beam_advance: the pool's lengths, parents and tokens", torch.int32, (G, W), *pool[1:])
-    _typed("beam_advance: lengths and done", torch.int32, (G,), lengths, done)
+    i32, f32, of, ow, each = torch.int32, torch.float32, scores.shape, pool.scores.shape, (G,)
+    if not (scores.dtype is f32 and pool.scores.dtype is f32 and ow[0] == G and parents.shape == of and tokens.shape == of and pool.lengths.shape == ow and pool.parents.shape == ow and
+            pool.tokens.shape == ow and lengths.shape == each and done.shape == each and
+            parents.dtype is tokens.dtype is pool.lengths.dtype is pool.parents.dtype is pool.tokens.dtype is lengths.dtype is done.dtype is i32):
+        raise KernelError(f"beam_advance: float32 scores and int32 of the rest, candidates {tuple(of)}, a pool [{G}, W], lengths and done [{G}]; got "
+                          f"{[(t.dtype, tuple(t.shape)) for t in (scores, parents, tokens, *pool, lengths, done)]}")
     if stop_ids is not None and stop_ids.dtype != torch.int32:
         raise KernelError("beam_advance: stop ids are int32")
-    i32, f32, dev = torch.int32, torch.float32, scores.device
+    dev = scores.device
     new = torch.empty(G, beams, dtype=i32, device=dev) if out.parents is None else out.parents
     res = BeamStep(torch.empty(G, beams, dtype=f32, device=dev) if out.scores is None else out.scores, new, torch.empty_like(new) if out.tokens is None else out.tokens,
                    torch.empty_like(lengths) if out.lengths is None else out.lengths, torch.empty_like(done) if out.done is None else out.done,
@@ -2759,7 +2760,7 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
     if new_slots is None:
         new_slots = torch.empty_like(slots)
     _typed("beam_reorder: new slots", torch.int32, (G * B,), new_slots)
-    about, made, read = [], [], {slots.data_ptr()}
+    about, made, read = [], [], {slots.data_ptr(), parents.data_ptr(), lens.data_ptr()}
     for (storage, table, stride), new in zip(paged, tables):
         if storage.dim() < 4 or stride < 1 or storage.element_size() < 2:
             raise KernelError(f"beam_reorder: a cache {storage.dtype} {tuple(storage.shape)}, an entry per {stride} tokens")
@@ -2836,9 +2837,8 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
         raise KernelError(f"step_tables: {columns} columns")
     if out is None:
         dev = q_lens.device
-        positions = torch.empty(T, dtype=torch.int32, device=dev)
-        out = StepTables(torch.empty(S + 1, dtype=torch.int32, device=dev), torch.empty_like(have), positions, torch.empty_like(positions),
-                         tuple(torch.empty(S, c, dtype=torch.int32, device=dev) for c in columns), tuple(torch.empty_like(positions) for _ in page_tables))
+        q_start, ctx_len, positions, seq_of_token, *maps = torch.empty(2 * S + 1 + (2 + n) * T, dtype=torch.int32, device=dev).split_with_sizes([S + 1, S] + [T] * (2 + n))
+        out = StepTables(q_start, ctx_len, positions, seq_of_token, tuple([torch.empty(S, c, dtype=torch.int32, device=dev) for c in columns]), tuple(maps))
     else:
         _typed("step_tables: out.q_start", torch.int32, (S + 1,), out.q_start)
         _typed("step_tables: out.ctx_len", torch.int32, (S,), out.ctx_len)

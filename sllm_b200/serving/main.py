@@ -180,6 +180,8 @@ def main(argv=None) -> int:
             for i, f in enumerate(found):
                 for r in f:
                     log("INFO", f"prompt {i}: {r.score:.4f} {r.finish_reason} {','.join(map(str, r.ids))}")
+            if not all(found):
+                raise SystemExit("sllm: the search found no continuation (no logit is a number above minus infinity)")
             results = [f[0] for f in found]
         else:
             results = llm.generate(prompts, params)

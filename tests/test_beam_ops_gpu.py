@@ -97,6 +97,32 @@ def test_candidates_far_apart_scores_and_large_logits():
     _check_candidates(x, scores, 24)
 
 
+@pytest.mark.parametrize("keep", [1, 7, 64, 128])
+@pytest.mark.parametrize("kind", ["rising", "falling", "level", "steps"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_candidates_of_long_whole_rows(keep, kind, dtype):
+    """More rows than the SMs hold blocks, so that each is read whole by one block, in all its runs: logits that rise through the row (every run finds more than its lists hold),
+    fall, are equal (the first tokens win), or rise in steps."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    G, B, V = 20, 31, 100003 if kind == "rising" else 100000
+    at = torch.arange(V, device=dev, dtype=torch.float64)
+    row = {"rising": at * 1e-4, "falling": -at * 1e-4, "level": at * 0 - 3.0, "steps": (at // 5000)}[kind].to(dtype)
+    logits = row[None].expand(G * B, V).contiguous()
+    scores = -torch.rand(G, B, device=dev, generator=torch.Generator(device=dev).manual_seed(keep)) * 1e-3
+    s, p, t = ops.beam_candidates(logits, scores, keep)
+    x = row.double()
+    best = torch.sort(x, descending=True, stable=True).indices[:keep]
+    lp = torch.log_softmax(x, 0)[best]
+    # all beams' rows are the same: s differs by the scores alone
+    value = (scores.double()[:, :, None] + lp[None, None]).reshape(G, B * keep)
+    order = torch.sort(value, dim=1, descending=True, stable=True).indices[:, :keep]
+    assert torch.equal(p.long(), order // keep) and torch.equal(t.long(), best[order % keep])
+    want = torch.gather(value, 1, order).cpu().numpy()
+    # (25 batches a thread in place of the 19 that SCORE counts: 6 additions more)
+    assert (np.abs(s.cpu().numpy() - want) <= SCORE(want) + 6 * 2.0 ** -24).all()
+
+
 def test_candidates_of_no_search():
     import sllm_b200.ops as ops
     dev = cuda_or_skip()
@@ -246,6 +272,26 @@ def test_reorder_leaves_alone_what_tables_do_not_name():
     assert torch.equal(kv, before) and torch.equal(state[0], held[1]) and tables[0].tolist() == [[1, 99], [1, 99]]
 
 
+def test_reorder_beyond_four_gigabytes():
+    """Rows of state and pages whose offsets pass 32 bits."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    n = 2_500_000_016
+    state = torch.empty(3, n, dtype=torch.uint8, device=dev)
+    for i in range(3):
+        state[i].fill_(7 + i)
+    kv = torch.zeros(2, 2, 70_000, 1, 16, 512, dtype=torch.bfloat16, device=dev)           # 4.6 GB
+    kv[:, :, 5], kv[:, :, 69_999] = 3.0, 1.0
+    # beam 2 has no child: beam 1 becomes a second child of beam 0 in beam 2's places
+    slots, tables = ops.beam_reorder(_i32([[0, 0, 1]], dev), _i32([0, 1, 2], dev), _i32([9], dev), states=[state], paged=[(kv, _i32([[5], [6], [69_999]], dev), 1)])
+    assert slots.tolist() == [0, 2, 1] and tables[0].tolist() == [[5], [69_999], [6]]
+    for row, value in ((0, 7), (1, 8), (2, 7)):
+        assert int(state[row].min()) == int(state[row].max()) == value
+    assert (kv[:, :, 69_999, :, :9] == 3).all() and (kv[:, :, 69_999, :, 9:] == 1).all() and (kv[:, :, 5] == 3).all() and not kv[:, :, 6].any()
+    del state, kv
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("S,most", [(1, 1), (1, 700), (5, 1), (48, 40), (300, 9), (1100, 2)])
 @pytest.mark.parametrize("grow", [False, True])
 @pytest.mark.parametrize("ps,strides", [(16, (1,)), (8, (1, 4)), (5, (1, 7, 3))])
@@ -341,3 +387,21 @@ def test_one_step_captured_and_replayed_on_another_stream():
         torch.cuda.current_stream().wait_stream(side)
         for a, b in zip(held, want):
             assert torch.equal(a, b)
+
+
+def test_two_streams_at_once_and_the_same_bits_every_time():
+    """Calls on two streams side by side have scratch of their own; lists that fill in any order give one result."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    g = torch.Generator(device=dev).manual_seed(11)
+    sets = [(torch.randn(6 * 4, 50021, device=dev, generator=g) * 3, -torch.rand(6, 4, device=dev, generator=g)) for _ in range(2)]
+    want = [ops.beam_candidates(x, s, 24) for x, s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for _ in range(20):
+        for (x, s), stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(ops.beam_candidates(x, s, 24))
+    torch.cuda.synchronize()
+    for i, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i % 2]))

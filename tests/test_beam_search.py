@@ -35,7 +35,7 @@ def beam_cpu_ops(cpu_ops, monkeypatch):
     return cpu_ops
 
 
-def _model(tmp_path, arch):
+def _model(tmp_path, arch, which="A"):
     """(folder, page size, vocabulary, logits behind a sequence of ids from the plain implementation)."""
     if arch == "qwen2":
         from tests.plain import qwen2_plain as m
@@ -45,7 +45,7 @@ def _model(tmp_path, arch):
         import importlib
         t = importlib.import_module(f"tests.test_{arch}")
         m = importlib.import_module(f"tests.plain.{arch}_plain")
-        config, page = t.CONFIGS["A"]
+        config, page = t.CONFIGS[which]
         d = t.make_model(tmp_path, config)
     cfg, w = m.load_model(d)
     order = {"qwen2": lambda ids: m.forward(ids, w, cfg), "gerupel": lambda ids: m.forward(cfg, w, ids)}.get(arch, lambda ids: m.forward(ids, cfg, w))
@@ -105,6 +105,50 @@ def test_search_of_every_architecture(tmp_path, arch, dev):
             assert not llm.engine.cache.requests
             llm.engine.cache.check()
             assert all(g.pool.used_count == 0 for g in llm.engine.cache.groups)
+
+
+@pytest.mark.parametrize("arch,which", [(a, "A") for a in ARCHITECTURES] + [("rososun", "only_delta"), ("nutopel", "only_gla"), ("sezopel", "retention"), ("gerupel", "odd")])
+def test_search_over_page_borders_with_freed_pages_poisoned(tmp_path, arch, which, dev, monkeypatch):
+    """Prompts that end at a page's border and just before it, continuations that fill pages, models without any page; pages nobody holds are full of NaN."""
+    monkeypatch.setenv("SLLM_POISON_FREED_PAGES", "1")
+    d, page, vocab, logits_of = _model(tmp_path, arch, which)
+    rng = np.random.default_rng(7)
+    prompts = [rng.integers(0, vocab, n).tolist() for n in (30, 16, 1)]
+    params = BeamParams(beams=3, max_new=19, length_penalty=0.0, results=3)
+    llm = _llm(d, page, dev, 9, 500)
+    for p, g in zip(prompts, llm.beam_search(prompts, params)):
+        _check(g, plain.search(logits_of, p, beams=3, max_new=19, power=0.0), p, logits_of, params, (arch, which, len(p)))
+    llm.engine.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("arch", ARCHITECTURES)
+def test_bfloat16_search_from_graphs_is_the_one_launch_by_launch(tmp_path, arch):
+    """The same kernels in the same order: the same bits, and what comes back is ordered and scored as bfloat16 logits allow."""
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    d, page, vocab, _ = _model(tmp_path, arch, "B" if arch not in ("qwen2", "rososun") else "A")
+    rng = np.random.default_rng(8)
+    prompts = [rng.integers(0, vocab, n).tolist() for n in (50, 9, 17, 33)]
+    params = BeamParams(beams=5, max_new=12, stop_ids=(int(vocab) - 1, 3), length_penalty=0.7)
+    got = [_llm(d, page, "cuda:0", 20, 600, dtype="bfloat16", cuda_graphs=g).beam_search(prompts, params) for g in (True, False)]
+    assert got[0] == got[1]
+    for g in got[0]:
+        assert 1 <= len(g) <= 5 and all(a.score >= b.score for a, b in zip(g, g[1:])) and all(np.isfinite(r.score) and len(r.ids) <= 12 for r in g)
+
+
+def test_parameters_changed_between_calls(tmp_path, dev):
+    """What was kept for one call's parameters is not taken for another's, though both are one object that the caller changes."""
+    d, page, vocab, logits_of = _model(tmp_path, "qwen2")
+    prompt = np.random.default_rng(2).integers(0, vocab, 11).tolist()
+    llm = _llm(d, page, dev, 4, 60)
+    params = BeamParams(beams=3, max_new=3)
+    for new, beams in ((3, 3), (6, 3), (3, 3), (4, 2), (3, 3), (5, 4), (2, 1), (7, 3), (3, 3)):
+        params.max_new, params.beams, params.results = new, beams, beams
+        _check(llm.beam_search([prompt], params)[0], plain.search(logits_of, prompt, beams=beams, max_new=new), prompt, logits_of, params, (new, beams))
+    params.beams = 40
+    with pytest.raises(ValueError):
+        llm.beam_search([prompt], params)
 
 
 def test_search_beside_running_requests_and_one_after_another(tmp_path, dev):
