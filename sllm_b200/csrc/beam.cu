@@ -7,8 +7,11 @@
 // logit, so a beam's own best are those of the largest logits, and no candidate of the search lies outside the `keep` best of its beam:
 //   beam_rows_kernel    a part of a row a block: the part's maximum, its sum of exponentials and its `keep` largest logits, from one pass over the logits;
 //   beam_merge_kernel   a block a search, a warp a beam: the beam's parts joined, then the beams.
-// Exponentials are float32, of float32 differences; their sums over a row's threads and parts, the logarithm and s are float64 (continuations
-// of different beams are compared with each other; of one beam by their logits alone).  s is rounded to float32 once, when it is stored.
+// Exponentials and a thread's sum of them are float32 (a few hundred terms, four sums a batch); the sums over threads and parts, the logarithm and s are float64, because continuations of
+// different beams are compared with each other (those of one beam by their logits alone).  s is rounded to float32 once, when it is stored.
+// Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 9.2 (0.4), 35 of 32,001 12 (0.7), 512 of 152,064 float32 61 (47.6) and
+// bfloat16 52 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
+// through side by side.
 #include "common.cuh"
 
 namespace sllm {
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
 }
 
 // A search: warp b joins the parts of beam b's row, then the first warp joins the beams.  Every step of a join takes the largest of the lists' heads, one a lane; the key behind a head
-// is loaded before the head goes.
+// is loaded before the head goes.  About 0.15 us a step of a chain that nothing hides: 4 us for 16 kept, 20 for 64.
 struct BeamHead {
   const unsigned long long* list;
   int at, n;
@@ -476,6 +479,7 @@ __global__ void beam_merge_kernel(const float* scores, const BeamPart* parts, co
 // so far; the first `beams` that are none go on.  At n = max_new what would go on is finished too.  The pool holds the W best finished ones in order (of equal
 // scores the earlier), lane w the w-th.  The search is over when nothing goes on, at max_new, or when the pool is full and the best that goes on cannot
 // get above its last: log-probabilities only fall, so it ends at best at best / max_new^power (power >= 0) or best / (n + 1)^power (power < 0).
+// A launch and its dependent loads bound it: 4 us for one search, 6.5 for 64 of 24 beams and 96 candidates (19 with a power an insertion; it is the same power for all of a step).
 struct BeamPool {
   float* score;
   int *length, *parent, *token;

@@ -4,10 +4,13 @@
 // Reordering.  Beam i of a search goes on from beam parents[i].  A parent's first child keeps the parent's state slot and the page the parent is writing; every
 // other child takes those of a beam that has no child, in order (there are as many), and only these are copied: 2 x (rows of state + written entries of a page) bytes are
 // read and written, which is what bounds it.  Whole pages are never written again, so a child's table names its parent's.  What is copied to had no child and what is copied from keeps
-// its place: no row is both, and the copies need no order among themselves.
+// its place: no row is both, and the copies need no order among themselves.  Every block works out who takes whose place for itself (a warp a search, votes); the copying is dealt over the blocks in
+// units.  Measured, us (what is copied, read and written once, at the measured copy rate): 16 rows of 16.8 MB of state 86 (82); a page of two beams in 24 layers 4.9 (0.04); pages of 32 beams in 28 layers of a 7B
+// model, 23.8 MB in pieces of 3 KB, 18 (7.3): a unit's look-ups of slots and pages are two dependent loads before its first copy.
 //
 // Step tables.  Request s brings q_lens[s] tokens behind have[s]; starts are sums over the requests before it, which every block that works for s adds up itself
-// (a thousand lengths are four a thread; a launch of its own for them would cost more).
+// (a thousand lengths are four a thread; a launch of its own for them would cost more).  Measured, us: 8 decoded tokens 2.7, 48 requests with 4,099 tokens in two groups and new pages 6.6, 512 requests
+// with 32,768 tokens and tables of 2,100 columns 7.0 (1.0 for its bytes): the sums and the look-ups, one after the other, bound it.
 #include "common.cuh"
 
 namespace sllm {
