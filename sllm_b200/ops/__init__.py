@@ -2721,20 +2721,29 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     if stop_ids is not None and stop_ids.dtype != torch.int32:
         raise KernelError("beam_advance: stop ids are int32")
     dev = scores.device
-    new = torch.empty(G, beams, dtype=i32, device=dev) if out.parents is None else out.parents
-    res = BeamStep(torch.empty(G, beams, dtype=f32, device=dev) if out.scores is None else out.scores, new, torch.empty_like(new) if out.tokens is None else out.tokens,
-                   torch.empty_like(lengths) if out.lengths is None else out.lengths, torch.empty_like(done) if out.done is None else out.done,
-                   BeamPool(*[torch.empty_like(a) if b is None else b for a, b in zip(pool, out.pool)]))
-    if out is not _NO_STEP:
+    if out is _NO_STEP:
+        if W == beams:                        # (views of one allocation cost less than allocations)
+            new_s, new_p, new_t, held_s, held_n, held_p, held_t = torch.empty(7, G, W, dtype=i32, device=dev).unbind(0)
+            res = BeamStep(new_s.view(f32), new_p, new_t, torch.empty_like(lengths), torch.empty_like(done), BeamPool(held_s.view(f32), held_n, held_p, held_t))
+        else:
+            new = torch.empty(G, beams, dtype=i32, device=dev)
+            res = BeamStep(torch.empty(G, beams, dtype=f32, device=dev), new, torch.empty_like(new), torch.empty_like(lengths), torch.empty_like(done),
+                           BeamPool(*[torch.empty_like(t) for t in pool]))
+    else:
+        new = torch.empty(G, beams, dtype=i32, device=dev) if out.parents is None else out.parents
+        res = BeamStep(torch.empty(G, beams, dtype=f32, device=dev) if out.scores is None else out.scores, new, torch.empty_like(new) if out.tokens is None else out.tokens,
+                       torch.empty_like(lengths) if out.lengths is None else out.lengths, torch.empty_like(done) if out.done is None else out.done,
+                       BeamPool(*[torch.empty_like(a) if b is None else b for a, b in zip(pool, out.pool)]))
         _typed("beam_advance: out.scores", f32, (G, beams), res.scores)
         _typed("beam_advance: out.parents and tokens", i32, (G, beams), res.parents, res.tokens)
         _typed("beam_advance: out.lengths and done", i32, (G,), res.lengths, res.done)
         _typed("beam_advance: out.pool", f32, (G, W), res.pool.scores)
         _typed("beam_advance: out.pool", i32, (G, W), *res.pool[1:])
     if G:
-        call("sllm_beam_advance", _p(scores), _p(parents), _p(tokens), G, keep, beams, W, *(_p(t) for t in pool), _p(lengths), _p(done),
-             _p(stop_ids), stop_ids.numel() if stop_ids is not None else 0, max_new, ctypes.byref(ctypes.c_double(power)),
-             _p(res.scores), _p(res.parents), _p(res.tokens), *(_p(t) for t in res.pool), _p(res.lengths), _p(res.done), _stream())
+        p, q = pool, res.pool
+        call("sllm_beam_advance", scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), G, keep, beams, W, p[0].data_ptr(), p[1].data_ptr(), p[2].data_ptr(), p[3].data_ptr(),
+             lengths.data_ptr(), done.data_ptr(), _p(stop_ids), stop_ids.numel() if stop_ids is not None else 0, max_new, ctypes.byref(ctypes.c_double(power)),
+             res[0].data_ptr(), res[1].data_ptr(), res[2].data_ptr(), q[0].data_ptr(), q[1].data_ptr(), q[2].data_ptr(), q[3].data_ptr(), res[3].data_ptr(), res[4].data_ptr(), _stream())
     return res
 
 
@@ -2815,15 +2824,15 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
     are written into its row of the page table; where the list is too short, -1.  ``out``: a `StepTables` of tensors to write."""
     page_tables = list(page_tables)
     n, T, page_size = len(page_tables), int(num_tokens), int(page_size)
-    strides = [1] * n if strides is None else [int(s) for s in strides]
+    strides = [1] * n if strides is None else list(map(int, strides))
     free = [None] * n if free is None else list(free)
     columns = [None] * n if columns is None else list(columns)
-    if len(strides) != n or len(free) != n or len(columns) != n or n > 8:
+    if not len(strides) == len(free) == len(columns) == n <= 8:
         raise KernelError(f"step_tables: {n} groups (8 at most), {len(strides)} strides, {len(free)} lists of free pages, {len(columns)} numbers of columns")
     flat = (q_lens, have, rows, *page_tables, *free) + ((*out[:4], *out.block_tables, *out.slot_mappings) if out is not None else ())
     _here("step_tables", *flat)
     S = q_lens.numel()
-    if S < 1 or T < 0 or page_size < 1 or any(s < 1 for s in strides):
+    if S < 1 or T < 0 or page_size < 1 or (n and min(strides) < 1):
         raise KernelError(f"step_tables: {S} requests, {T} tokens, pages of {page_size}, strides {strides}")
     _typed("step_tables: lengths", torch.int32, (S,), q_lens, have)
     if rows is not None:
@@ -2835,7 +2844,7 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
         if f is not None and (f.dtype != torch.int32 or f.dim() != 1):
             raise KernelError("step_tables: free pages are an int32 list")
     columns = [t.shape[1] if c is None else int(c) for t, c in zip(page_tables, columns)]
-    if any(c < 0 for c in columns):
+    if n and min(columns) < 0:
         raise KernelError(f"step_tables: {columns} columns")
     if out is None:
         dev = q_lens.device
@@ -2849,13 +2858,13 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
             raise KernelError("step_tables: out has other groups")
         for t, c in zip(out.block_tables, columns):
             _typed("step_tables: out.block_tables", torch.int32, (S, c), t)
-        read = {t.data_ptr() for t in (q_lens, have, *page_tables) if t.numel()}
+        read = {t.data_ptr() for t in (q_lens, have, rows, *page_tables, *free) if t is not None and t.numel()}
         if any(t.numel() and t.data_ptr() in read for t in (*out[:4], *out.block_tables, *out.slot_mappings)):
             raise KernelError("step_tables: what is written cannot be what is read")
     about = []
     for t, f, c, st, b, m in zip(page_tables, free, columns, strides, out.block_tables, out.slot_mappings):
         # (an empty list of free pages is still a list: its pointer only has to be one)
         about += (t.data_ptr(), 0 if f is None else (f.data_ptr() or t.data_ptr()), b.data_ptr(), m.data_ptr(), t.shape[1], c, 0 if f is None else f.numel(), st)
-    call("sllm_step_tables", _p(q_lens), _p(have), _p(rows), S, N, T, page_size, _p(out.q_start), _p(out.ctx_len), _p(out.positions), _p(out.seq_of_token),
+    call("sllm_step_tables", q_lens.data_ptr(), have.data_ptr(), _p(rows), S, N, T, page_size, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
          (ctypes.c_longlong * len(about))(*about), n, _stream())
     return out
