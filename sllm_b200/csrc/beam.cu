@@ -395,75 +395,133 @@ struct BeamHead {
   }
 };
 
-__global__ void beam_merge_kernel(const float* scores, const BeamPart* parts, const unsigned long long* keys, int B, int keep, int splits, float* out_score, int* out_parent,
-                                  int* out_token) {
+// Neighbours in the order that are two beams' and lie closer than this are told apart by the beams' sums in 64 bits throughout, which the block makes from the rows then (the parts' sums are good
+// to some 2^-25; a search of 8 beams meets this once in hundreds of calls, and a row of 152,064 takes it 60 us).
+constexpr double BEAM_CLOSE = 2.384185791015625e-7;           // 2^-22
+
+template <typename T>
+__global__ void beam_merge_kernel(const T* logits, int V, const float* scores, const BeamPart* parts, const unsigned long long* keys, int B, int keep, int splits, float* out_score,
+                                  int* out_parent, int* out_token) {
   extern __shared__ __align__(16) unsigned char beam_smem[];
   unsigned long long* lists = reinterpret_cast<unsigned long long*>(beam_smem);        // [B][splits][keep]: a beam's parts
   unsigned long long* merged = lists + (size_t)B * splits * keep;                      // [B][keep]: a beam's keys joined, then its scores
   int* best_token = reinterpret_cast<int*>(merged + B * keep);                         // [B][keep]
+  float* best_logit = reinterpret_cast<float*>(best_token + B * keep);                 // [B][keep]
+  __shared__ int picked[BEAM_KEEP];                                                    // beam << 8 | place
+  __shared__ unsigned close_s;
+  __shared__ double red[BEAM_MAX];
   pdl_launch_dependents();
   pdl_wait();
   const int g = blockIdx.x, b = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t row = (size_t)g * B + b;
-  {
-    const float score = scores[row];
-    unsigned long long *mine = lists + (size_t)b * splits * keep, *joined = merged + b * keep;
-    const unsigned long long* src = keys + row * splits * keep;
-    const BeamPart part = lane < splits ? parts[row * splits + lane] : BeamPart{0.0, -INFINITY};
+  const float score = scores[row];
+  unsigned long long *mine = lists + (size_t)b * splits * keep, *joined = merged + b * keep;
+  const unsigned long long* src = keys + row * splits * keep;
+  const BeamPart part = lane < splits ? parts[row * splits + lane] : BeamPart{0.0, -INFINITY};
 #pragma unroll 4
-    for (int i = lane; i < splits * keep; i += 32) mine[i] = src[i];
-    const float top = warp_max(part.max);
-    double sum = 0.0;
-    if (part.max > -INFINITY && (top < INFINITY || part.max == top)) sum = part.max == top ? part.sum : part.sum * exp((double)part.max - (double)top);
-    if (splits > 1) {
+  for (int i = lane; i < splits * keep; i += 32) mine[i] = src[i];
+  const float top = warp_max(part.max);
+  double sum = 0.0;
+  if (part.max > -INFINITY && (top < INFINITY || part.max == top)) sum = part.max == top ? part.sum : part.sum * exp((double)part.max - (double)top);
+  if (splits > 1) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    } else {
-      sum = __shfl_sync(0xffffffffu, sum, 0);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  } else {
+    sum = __shfl_sync(0xffffffffu, sum, 0);
+  }
+  __syncwarp();
+  int found = 0;
+  if (splits > 1) {                                 // lane l walks the l-th part's list
+    BeamHead h(mine + lane * keep, lane < splits ? keep : 0);
+    for (; found < keep; ++found) {
+      const unsigned long long best = warp_max_key(h.head);
+      if (best == 0) break;
+      if (h.head == best) {
+        joined[found] = best;
+        h.pop();
+      }
     }
     __syncwarp();
-    int n = 0;
-    if (splits > 1) {                               // lane l walks the l-th part's list
-      BeamHead h(mine + lane * keep, lane < splits ? keep : 0);
-      for (; n < keep; ++n) {
+  } else {
+    joined = mine;
+    found = keep;
+  }
+  const bool alive = score > -INFINITY && top > -INFINITY;
+  auto score_of = [&](float x, double lse) { return (double)score + ((x == top ? 0.0 : (double)x - (double)top) - lse); };
+  const double lse = log(sum);
+  for (int i = lane; i < keep; i += 32) {
+    const unsigned long long k = i < found && alive ? joined[i] : 0ull;
+    const float x = beam_value((uint32_t)(k >> 32));
+    const double v = score_of(x, lse);
+    merged[b * keep + i] = k != 0 && v > -INFINITY ? order_double(v) : 0ull;
+    best_token[b * keep + i] = (int)~(uint32_t)k;
+    best_logit[b * keep + i] = x;
+  }
+  int n = 0;
+  for (bool again = false;; again = true) {
+    __syncthreads();
+    if (b == 0) {
+      // (what is picked is noted and written out by all lanes afterwards: a step of the join is a chain that nothing hides)
+      BeamHead h(merged + lane * keep, lane < B ? keep : 0);
+      for (n = 0; n < keep; ++n) {
         const unsigned long long best = warp_max_key(h.head);
         if (best == 0) break;
-        if (h.head == best) {
-          joined[n] = best;
+        const unsigned here = __ballot_sync(0xffffffffu, h.head == best);
+        if ((here & ((2u << lane) - 1)) == 1u << lane) {                       // of equal scores the first beam's
+          picked[n] = lane << 8 | (h.at - 2);
           h.pop();
         }
       }
       __syncwarp();
-    } else {
-      joined = mine;
-      n = keep;
+      // the beams with one that is left out as close to the last that is not
+      const double last = n > 0 ? double_of(merged[(picked[n - 1] >> 8) * keep + (picked[n - 1] & 255)]) : 0.0;
+      const unsigned behind = __ballot_sync(0xffffffffu, n > 0 && h.head != 0 && last - double_of(h.head) < BEAM_CLOSE);
+      unsigned close = 0;
+      for (int i = lane; i < n; i += 32) {
+        const int a = picked[i] >> 8;
+        const double v = double_of(merged[a * keep + (picked[i] & 255)]);
+        if (i + 1 < n) {
+          const int c = picked[i + 1] >> 8;
+          if (a != c && v - double_of(merged[c * keep + (picked[i + 1] & 255)]) < BEAM_CLOSE) close |= 1u << a | 1u << c;
+        } else if (behind & ~(1u << a)) {
+          close |= 1u << a | behind;
+        }
+      }
+      close = __reduce_or_sync(0xffffffffu, close);
+      if (lane == 0) close_s = again ? 0u : close;
     }
-    const bool alive = score > -INFINITY && top > -INFINITY;
-    const double lse = log(sum);
-    for (int i = lane; i < keep; i += 32) {
-      const unsigned long long k = i < n && alive ? joined[i] : 0ull;
-      const float x = beam_value((uint32_t)(k >> 32));
-      const double v = (double)score + ((x == top ? 0.0 : (double)x - (double)top) - lse);
-      merged[b * keep + i] = k != 0 && v > -INFINITY ? order_double(v) : 0ull;
-      best_token[b * keep + i] = (int)~(uint32_t)k;
+    __syncthreads();
+    const unsigned close = close_s;
+    if (close == 0) break;
+    for (unsigned left = close; left; left &= left - 1) {
+      const int c = __ffs(left) - 1;
+      if (b == c && lane == 0) red[0] = (double)top;
+      __syncthreads();
+      const double c_top = red[0];
+      __syncthreads();
+      if (!(c_top < INFINITY)) continue;            // (an infinite maximum: a count, which is exact)
+      const T* x_row = logits + ((size_t)g * B + c) * V;
+      double all = 0.0;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < V; i += blockDim.x) {
+        const float x = to_f32(x_row[i]);
+        if (x > -INFINITY) all += exp((double)x - c_top);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      if (lane == 0) red[b] = all;
+      __syncthreads();
+      if (b == c) {
+        double total = 0.0;
+        for (int w = 0; w < B; ++w) total += red[w];
+        const double exact = log(total);
+        for (int i = lane; i < keep; i += 32)
+          if (merged[c * keep + i] != 0) merged[c * keep + i] = order_double(score_of(best_logit[c * keep + i], exact));
+      }
+      __syncthreads();
     }
   }
-  __syncthreads();
   if (b != 0) return;
-  // what is picked is noted as beam << 8 | place and written out by all lanes afterwards: a step of the join is a chain that nothing hides
-  int* picked = reinterpret_cast<int*>(lists);
-  BeamHead h(merged + lane * keep, lane < B ? keep : 0);
-  int n = 0;
-  for (; n < keep; ++n) {
-    const unsigned long long best = warp_max_key(h.head);
-    if (best == 0) break;
-    const unsigned here = __ballot_sync(0xffffffffu, h.head == best);
-    if ((here & ((2u << lane) - 1)) == 1u << lane) {                           // of equal scores the first beam's
-      picked[n] = lane << 8 | (h.at - 2);
-      h.pop();
-    }
-  }
-  __syncwarp();
   for (int i = lane; i < keep; i += 32) {
     const size_t o = (size_t)g * keep + i;
     const int which = i < n ? picked[i] : 0, from = (which >> 8) * keep + (which & 255);
@@ -593,7 +651,7 @@ __global__ void __launch_bounds__(32) beam_advance_kernel(const float* c_score, 
   }
 }
 
-static size_t beam_merge_smem(int B, int splits, int keep) { return (size_t)B * keep * (8 * splits + 12); }
+static size_t beam_merge_smem(int B, int splits, int keep) { return (size_t)B * keep * (8 * splits + 16); }
 
 static int beam_log2_lanes(int keep) {             // four groups a wanted key, where the threads suffice
   int lg = 5;
@@ -602,12 +660,15 @@ static int beam_log2_lanes(int keep) {             // four groups a wanted key, 
 }
 
 template <typename T>
-static bool beam_rows(const T* logits, int rows, int V, int keep, int splits, BeamPart* parts, unsigned long long* keys, cudaStream_t stream) {
-  static SharedLimit limit;
+static bool beam_both(const T* logits, const float* scores, int G, int B, int V, int keep, int splits, BeamPart* parts, unsigned long long* keys, float* out_score, int* out_parent,
+                      int* out_token, cudaStream_t stream) {
+  static SharedLimit rows_limit, merge_limit;
   constexpr int N = BeamLoad<T>::N;
-  if (!limit.raise(beam_rows_kernel<T>, sizeof(BeamShared))) return false;
-  launch_kernel(beam_rows_kernel<T>, dim3((unsigned)(rows * splits)), BEAM_THREADS, sizeof(BeamShared), stream, logits, V, keep, beam_log2_lanes(keep), splits,
+  const size_t merge_smem = beam_merge_smem(B, splits, keep);
+  if (!rows_limit.raise(beam_rows_kernel<T>, sizeof(BeamShared)) || !merge_limit.raise(beam_merge_kernel<T>, merge_smem)) return false;
+  launch_kernel(beam_rows_kernel<T>, dim3((unsigned)(G * B * splits)), BEAM_THREADS, sizeof(BeamShared), stream, logits, V, keep, beam_log2_lanes(keep), splits,
                 ((V + N - 1) / N + splits - 1) / splits, parts, keys);
+  launch_kernel(beam_merge_kernel<T>, G, 32 * B, merge_smem, stream, logits, V, scores, (const BeamPart*)parts, (const unsigned long long*)keys, B, keep, splits, out_score, out_parent, out_token);
   return true;
 }
 
@@ -639,16 +700,12 @@ SLLM_EXPORT int sllm_beam_candidates(const void* logits, int dtype, const float*
   if (G == 0) return SLLM_OK;
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(scratch);
   BeamPart* parts = reinterpret_cast<BeamPart*>(keys + (size_t)G * B * splits * keep);
-  static SharedLimit limit;
-  const size_t merge_smem = beam_merge_smem(B, splits, keep);
-  bool there = limit.raise(beam_merge_kernel, merge_smem);
-  if (dtype == SLLM_F32) there = there && beam_rows((const float*)logits, G * B, V, keep, splits, parts, keys, stream);
-  else there = there && beam_rows((const __nv_bfloat16*)logits, G * B, V, keep, splits, parts, keys, stream);
+  const bool there = dtype == SLLM_F32 ? beam_both((const float*)logits, scores, G, B, V, keep, splits, parts, keys, out_score, out_parent, out_token, stream)
+                                       : beam_both((const __nv_bfloat16*)logits, scores, G, B, V, keep, splits, parts, keys, out_score, out_parent, out_token, stream);
   if (!there) {
     set_error("beam_candidates: cannot raise the shared memory limit");
     return SLLM_ERR_LAUNCH;
   }
-  launch_kernel(beam_merge_kernel, G, 32 * B, merge_smem, stream, scores, (const BeamPart*)parts, (const unsigned long long*)keys, B, keep, splits, out_score, out_parent, out_token);
   return launch_status("beam_candidates");
 }
 

@@ -97,6 +97,25 @@ def test_candidates_far_apart_scores_and_large_logits():
     _check_candidates(x, scores, 24)
 
 
+@pytest.mark.parametrize("V", [40, 3001, 50000])
+@pytest.mark.parametrize("keep", [1, 2, 3, 9])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_beams_whose_best_lie_next_to_each_other(V, keep, dtype):
+    """Scores drawn so that the beams' best continuations are equal to some 1e-9, closer than float32 exponentials tell: the order is that of the sums in 64 bits, at the cut too."""
+    dev = cuda_or_skip()
+    G, B = 40, 3
+    g = torch.Generator(device=dev).manual_seed(V + keep)
+    logits = (torch.randn(G * B, V, device=dev, generator=g) * 2).to(dtype)
+    x = logits.double().reshape(G, B, V)
+    best = x.amax(2) - torch.logsumexp(x, 2)
+    scores = (best[:, :1] - best).float()
+    gaps = (scores.double() + best - best[:, :1]).abs()
+    assert gaps.max() < 2e-7                                  # (half a step of scores below 4)
+    if keep == 9:
+        scores[::2, 2] = -math.inf                            # two of them
+    _check_candidates(logits, scores.contiguous(), keep)
+
+
 @pytest.mark.parametrize("keep", [1, 7, 64, 128])
 @pytest.mark.parametrize("kind", ["rising", "falling", "level", "steps"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
