@@ -9,8 +9,8 @@
 //   beam_merge_kernel   a block a search, a warp a beam: the beam's parts joined, then the beams.
 // Exponentials and a thread's sum of them are float32 (a few hundred terms, four sums a batch); the sums over threads and parts, the logarithm and s are float64, because continuations of
 // different beams are compared with each other (those of one beam by their logits alone).  s is rounded to float32 once, when it is stored.
-// Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 9.2 (0.4), 35 of 32,001 12 (0.7), 512 of 152,064 float32 61 (47.6) and
-// bfloat16 52 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
+// Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 9.9 (0.4), 35 of 32,001 12.7 (0.7), 512 of 152,064 float32 62 (47.6) and
+// bfloat16 53 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
 // through side by side.
 #include "common.cuh"
 
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
 }
 
 // A search: warp b joins the parts of beam b's row, then the first warp joins the beams.  Every step of a join takes the largest of the lists' heads, one a lane; the key behind a head
-// is loaded before the head goes.  About 0.15 us a step of a chain that nothing hides: 4 us for 16 kept, 20 for 64.
+// is loaded before the head goes.  About 0.15 us a step of a chain that nothing hides: 5 us for 16 kept, 20 for 64.
 struct BeamHead {
   const unsigned long long* list;
   int at, n;
