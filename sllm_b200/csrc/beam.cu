@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
   const int row = blockIdx.x / splits, part = blockIdx.x - row * splits;
   const T* x_row = logits + (size_t)row * V;
   // Pieces of 16 bytes of tokens.  Which thread takes which tokens goes by their numbers and not by where the row lies, so that equal rows give equal sums; a row that does not begin
-  // on 16 bytes is read an element at a time (from L1 but for the first of a piece).
+  // on 16 bytes is read an element at a time (from L1 but for the first of a piece; 512 rows of 152,063: float32 76 us for 62, bfloat16 83 for 53).
   const int pieces = (V + N - 1) / N;
   const int v0 = part * part_vecs, v1 = min(v0 + part_vecs, pieces);
   const int whole = (reinterpret_cast<uintptr_t>(x_row) & 15) == 0 ? min(v1, V / N) : 0;          // pieces that are read as they lie
