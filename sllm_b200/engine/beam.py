@@ -51,6 +51,7 @@ class _Searches:
         self.live = torch.zeros(layout.total, dtype=torch.int32, device=engine.device)
         self.next = torch.zeros_like(self.live)
         self.ones = torch.ones(R, dtype=torch.int32, device=engine.device)
+        self.first = torch.zeros((G, B), dtype=torch.int32, device=engine.device)
         self.stop_ids = torch.tensor(params.stop_ids, dtype=torch.int32, device=engine.device) if params.stop_ids else None
         self.ctx = context(layout, self.live, cache.page_size, [1] * R, [bucket] * R, is_graph_replay=pin)
         self.ctx.token_ids = layout.sec(self.live, "tokens")
@@ -92,14 +93,15 @@ class _Searches:
         self.next.copy_(self.host, non_blocking=True)
         engine.h2d_bytes += self.host.numel() * 4
 
-    def choose(self, logits, scores) -> None:
-        """From the logits behind every beam to the next step's description."""
+    def choose(self, logits, scores, behind_prompt: bool = False) -> None:
+        """From the logits behind every beam to the next step's description.  Behind the prompt every beam goes on from the first, which alone holds it: also those of a search that is
+        over or has too few candidates, which are run forward beside the others like any row."""
         p, (step, slots, pages, tables) = self.params, self.now
         made, new_slots, new_pages, new_tables = self.then
         found = ops.beam_candidates(logits, scores, p.keep)
         ops.beam_advance(*found, step.pool, step.lengths, step.done, beams=p.beams, stop_ids=self.stop_ids, max_new=p.max_new,
                          length_penalty=p.length_penalty, out=made)
-        ops.beam_reorder(made.parents, slots, tables.ctx_len, states=self.states,
+        ops.beam_reorder(self.first if behind_prompt else made.parents, slots, tables.ctx_len, states=self.states,
                          paged=[(s, t, st) for s, t, st in zip(self.storage, pages, self.strides)], out=(new_slots, new_pages))
         ops.step_tables(self.ones, tables.ctx_len, new_pages, page_size=self.page_size, num_tokens=self.R, strides=self.strides, out=new_tables)
         self.live.copy_(self.next)
@@ -241,7 +243,7 @@ class BeamSearch:
             lo = s.layout.offs["done"] - a
             return bool(back[t, lo:lo + G].all())
         # before the first token there is one beam a search, of score 0
-        s.choose(logits, torch.zeros((G, 1), dtype=torch.float32, device=eng.device))
+        s.choose(logits, torch.zeros((G, 1), dtype=torch.float32, device=eng.device), behind_prompt=True)
         note(0)
         steps = 1
         while steps < params.max_new:

@@ -121,6 +121,48 @@ def test_search_over_page_borders_with_freed_pages_poisoned(tmp_path, arch, whic
     llm.engine.cache.check()
 
 
+@pytest.mark.parametrize("arch", ARCHITECTURES)
+def test_rows_of_a_search_that_is_over_at_once_hold_its_prompt(tmp_path, arch, dev, monkeypatch):
+    """A search whose likeliest first token is a stop, with one result wanted, is over before its other beams held anything.  Their rows run on beside the other search: over pages that are
+    theirs or the prompt's, and over numbers (pages nobody holds are full of NaN here)."""
+    import sllm_b200.ops as ops
+    monkeypatch.setenv("SLLM_POISON_FREED_PAGES", "1")
+    d, page, vocab, logits_of = _model(tmp_path, arch)
+    rng = np.random.default_rng(12)
+    prompts = [rng.integers(0, vocab, n).tolist() for n in (2 * page + 5, 7)]
+    stop = int(np.argmax(logits_of(prompts[0])))
+    params = BeamParams(beams=3, max_new=6, stop_ids=(stop,), results=1, length_penalty=0.0)       # (no later one can score above the best first)
+    seen, logits_seen, tables_of, candidates = [], [], ops.step_tables, ops.beam_candidates
+
+    def step_tables(q_lens, have, pages, **kw):
+        made = tables_of(q_lens, have, pages, **kw)
+        if not (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
+            seen.append([(made.ctx_len.cpu().clone(), [t.cpu().clone() for t in made.block_tables], kw["strides"], kw["page_size"])])
+        return made
+
+    def beam_candidates(logits, scores, keep):
+        if logits.shape[0] > len(prompts):
+            logits_seen.append(logits.float().cpu().clone())
+        return candidates(logits, scores, keep)
+    monkeypatch.setattr(ops, "step_tables", step_tables)
+    monkeypatch.setattr(ops, "beam_candidates", beam_candidates)
+    llm = _llm(d, page, dev, 6, 300, cuda_graphs=False)
+    got = llm.beam_search(prompts, params)
+    assert seen and logits_seen
+    windows = any(g.need.window for g in llm.engine.cache.groups)
+    for step, in seen:
+        ctx, tables, strides, ps = step
+        for table, stride in zip(tables, strides):
+            for r, n in enumerate(ctx.tolist()):
+                assert windows or (table[r, :-(-(n // stride) // ps)] >= 0).all(), (arch, r, n, table[r])
+    for x in logits_seen:
+        assert not torch.isnan(x).any(), arch
+    assert got[0][0].ids == [] and got[0][0].finish_reason == "stop"
+    for p, g in zip(prompts, got):
+        _check(g, plain.search(logits_of, p, beams=3, max_new=6, stop_ids=(stop,), power=0.0, width=1), p, logits_of, params, (arch, len(p)))
+    llm.engine.cache.check()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("arch", ARCHITECTURES)
 def test_bfloat16_search_from_graphs_is_the_one_launch_by_launch(tmp_path, arch):
