@@ -634,7 +634,7 @@ static int launch_ta(const CUtensorMap& mk, const CUtensorMap& mv, const CUtenso
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = pdl_allowed(stream) ? 2 : 1;
     cudaLaunchKernelEx(&cfg, attention_tma_decode_kernel<HD, CAP, REL>, mk, mv, rk, rv, p);
     return launch_status("attention_tma");
   }

@@ -143,7 +143,11 @@ __device__ __forceinline__ float4 load_now_l2(const float4* p) {
   return v;
 }
 
-bool pdl_enabled();
+// Whether a launch on this stream may have the attribute: not where it is off, and not where the launch before made a step's description (lengths, block tables), which the attention
+// kernels read before their wait.  `pdl_description_made` says so behind such a launch; the next one of this library on the stream then begins when everything before it has completed and
+// is visible, and with it all that follow.
+bool pdl_allowed(cudaStream_t stream);
+void pdl_description_made(cudaStream_t stream);
 int num_sms();           // streaming multiprocessors of the current device (asked once per device)
 
 template <typename... KArgs, typename... Args>
@@ -158,7 +162,7 @@ inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = pdl_allowed(stream) ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);   // errors are read by launch_status()
 }
 

@@ -5,6 +5,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace sllm {
@@ -15,12 +17,52 @@ void set_error(const char* msg) {
   g_error[sizeof g_error - 1] = 0;
 }
 
-bool pdl_enabled() {
+static bool pdl_enabled() {
   static const bool on = [] {
     const char* v = getenv("SLLM_PDL");
     return !(v && v[0] == '0');
   }();
   return on;
+}
+
+// The streams whose last launch of this library made a step's description, by device and handle (handle 0 is a stream of every device).  Fixed places: nothing is allocated, nothing can fail;
+// where they are all taken every launch from then on is a plain one.  A stream that was destroyed with its mark set leaves a mark, which costs a later stream of the same handle one plain launch.
+namespace {
+constexpr int DESCRIBED_MOST = 256;
+struct Described {
+  int device;
+  cudaStream_t stream;
+} described[DESCRIBED_MOST];
+std::mutex described_mutex;
+std::atomic<int> described_count{0};           // read without the lock by every launch; > DESCRIBED_MOST: no places were left
+}  // namespace
+
+void pdl_description_made(cudaStream_t stream) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(described_mutex);
+  const int n = described_count.load(std::memory_order_relaxed);
+  for (int i = 0; i < n && i < DESCRIBED_MOST; ++i)
+    if (described[i].device == dev && described[i].stream == stream) return;
+  if (n < DESCRIBED_MOST) described[n] = Described{dev, stream};
+  if (n <= DESCRIBED_MOST) described_count.store(n + 1, std::memory_order_release);
+}
+
+bool pdl_allowed(cudaStream_t stream) {
+  if (!pdl_enabled()) return false;
+  if (described_count.load(std::memory_order_acquire) == 0) return true;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(described_mutex);
+  const int n = described_count.load(std::memory_order_relaxed);
+  if (n > DESCRIBED_MOST) return false;
+  for (int i = 0; i < n; ++i)
+    if (described[i].device == dev && described[i].stream == stream) {
+      described[i] = described[n - 1];
+      described_count.store(n - 1, std::memory_order_release);
+      return false;
+    }
+  return true;
 }
 
 int num_sms() {

@@ -311,7 +311,7 @@ static int launch_clusters(Kernel kernel, dim3 grid, int threads, int smem, dim3
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = pdl_allowed(stream) ? 2 : 1;
   cudaLaunchKernelEx(&cfg, kernel, A, W, bias, C, M, N, K, S, seg);
   return launch_status("gemm_f32");
 }

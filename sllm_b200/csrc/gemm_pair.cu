@@ -547,7 +547,7 @@ static void pair_launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&at
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = pdl_allowed(stream) ? 2 : 1;
 }
 
 template <int EPI, int R2>

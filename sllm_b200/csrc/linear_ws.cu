@@ -562,7 +562,7 @@ static int launch_ws(const __nv_bfloat16* x, const __nv_bfloat16* W, const float
       attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
       attr[1].val.programmaticStreamSerializationAllowed = 1;
       cfg.attrs = attr;
-      cfg.numAttrs = pdl_enabled() ? 2 : 1;
+      cfg.numAttrs = pdl_allowed(stream) ? 2 : 1;
       cudaLaunchKernelEx(&cfg, ws_kernel<NT, EPI, OUT, false, WS_SLICED>(), x, W, bias, (OUT*)out, residual, M, N, K, rope, norm, act, token, slices);
       return launch_status("linear_ws");
     }

@@ -1022,7 +1022,7 @@ static void sample_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = 1;                             // (the launch says whether it takes the second)
 }
 
 // Raises the kernel's limit of shared memory; what fits the GPU is asked with it raised, whichever call of a process comes first.
@@ -1043,7 +1043,6 @@ static int row_blocks_log2(int R, int V) {
         cudaLaunchConfig_t cfg;
         cudaLaunchAttribute attr[2];
         sample_config(cfg, attr, num_sms(), 1 << lg, SAMPLE_SMEM, nullptr);
-        cfg.numAttrs = 1;
         if (cudaOccupancyMaxActiveClusters(&rows[lg], sample_rows_kernel, &cfg) != cudaSuccess) rows[lg] = 0;
       }
       cudaGetLastError();
@@ -1084,6 +1083,7 @@ SLLM_EXPORT int sllm_sample_rows(const float* logits, int R, int V, const float*
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
   sample_config(cfg, attr, R, 1 << lg, smem, stream);
+  cfg.numAttrs = pdl_allowed(stream) ? 2 : 1;
   cudaLaunchKernelEx(&cfg, sample_rows_kernel, logits, V, temperature, uniform, top_k, top_p, out, lg);
   return launch_status("sample_rows");
 }

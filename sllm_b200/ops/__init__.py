@@ -12,6 +12,8 @@ then: what belongs to a model (matrices, gains, biases, tables of angles and of 
 function, and the step's description (tiles, lengths, block tables) in the attention functions.  A
 program that computes one of these on the device puts a copy, an event or a synchronisation between
 that and the first call here; the engine's are loaded, or copied from the host, before a step begins.
+(What `step_tables` and `beam_reorder` make is in place without that: the launch behind either on its
+stream waits until it is.)
 Everything else, token ids, positions and slots among it, may come from the kernel just before.
 """
 
@@ -2756,7 +2758,8 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
     of the row and of the page's entries, in the slots and pages of beams without a child, in order; pages before that one are shared, those behind it stay each
     beam's own.  A beam with parent -1 takes such a place as it is.  Each slot, and each page from the first that is partly written on, belongs to one beam.
 
-    Returns ``(new slots, [new block tables])``; ``out`` is such a pair of tensors to write (others than those read).  At most 32 beams a search, 2,048 in all."""
+    Returns ``(new slots, [new block tables])``; ``out`` is such a pair of tensors to write (others than those read).  At most 32 beams a search, 2,048 in all.
+    Any function may take the results next on the same stream, attention too."""
     states, paged = list(states), [(s, t, int(st)) for s, t, st in paged]
     new_slots, tables = out if out is not None else (None, [None] * len(paged))
     _here("beam_reorder", parents, slots, lens, *states, *(x for p in paged for x in p[:2]), new_slots, *tables)
@@ -2821,7 +2824,8 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
     requests bring, the rows behind them have position 0, request 0 and slot -1; with fewer, tokens are left out.
 
     ``free`` (int32 ``[n]`` per group): pages that nobody holds.  A request whose new tokens need further pages takes them from there, in the order of the requests, and they
-    are written into its row of the page table; where the list is too short, -1.  ``out``: a `StepTables` of tensors to write."""
+    are written into its row of the page table; where the list is too short, -1.  ``out``: a `StepTables` of tensors to write.
+    Any function may take the results next on the same stream, attention too."""
     page_tables = list(page_tables)
     n, T, page_size = len(page_tables), int(num_tokens), int(page_size)
     strides = [1] * n if strides is None else list(map(int, strides))

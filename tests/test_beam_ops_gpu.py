@@ -1,6 +1,7 @@
 """The operators of a beam search against their definitions in float64 (tests/plain/beam_plain.py).  Whole numbers are equal; scores are float32 roundings of a float64 sum whose
 only float32 part are the exponentials, see `SCORE`."""
 
+import itertools
 import math
 
 import numpy as np
@@ -424,3 +425,70 @@ def test_two_streams_at_once_and_the_same_bits_every_time():
     torch.cuda.synchronize()
     for i, r in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(r, want[i % 2]))
+
+
+@pytest.mark.parametrize("written", [False, True], ids=["tables", "tables-write"])
+@pytest.mark.parametrize("form", ["tma", "mma", "simt"])
+@pytest.mark.parametrize("source", ["tables", "reorder"])
+def test_attention_right_behind_the_operators_that_make_its_tables(form, written, source):
+    """Attention reads lengths and block tables before it waits for the kernel before; what `step_tables` and `beam_reorder` made is there all the same, launch by launch and in a graph.  The tensors
+    written are the same ones every turn, so that what lay there before would be another turn's pages."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    S, nq, nkv, hd, ps, columns = 4, 8, 2, 128, 16, 12
+    pages = 3 * S * columns
+    g = torch.Generator(device=dev).manual_seed(2)
+    kv0 = torch.randn(2, pages, nkv, ps, hd, device=dev, generator=g).bfloat16()
+    kv = kv0.clone()
+    qkv = torch.randn(S, (nq + 2 * nkv) * hd, device=dev, generator=g).bfloat16()
+    q = qkv[:, :nq * hd].contiguous()
+    rng = np.random.default_rng(2)
+    sets = [(_i32(rng.permutation(pages)[:S * columns].reshape(S, columns), dev), _i32(rng.integers(1, ps * columns - 2, 2).repeat(2), dev), _i32([rng.permutation(2).tolist() for _ in range(2)], dev))
+            for _ in range(6)]
+    q_lens, slots = _i32([1] * S, dev), _i32(range(S), dev)
+    now = [x.clone() for x in sets[0]]
+    empty = lambda *n: torch.zeros(n, dtype=torch.int32, device=dev)                                 # noqa: E731
+    out = ops.StepTables(empty(S + 1), empty(S), empty(S), empty(S), (empty(S, columns),), (empty(S),))
+    mine = (empty(S), [empty(S, columns)])
+    tiles, _ = ops.attention_tiles([1] * S, nq // nkv, dev)
+    result = torch.empty_like(q)
+
+    def turn(wait):
+        t = ops.step_tables(q_lens, now[1], [now[0]], page_size=ps, num_tokens=S, out=out)
+        wait()
+        bt = t.block_tables[0]
+        if source == "reorder":
+            bt = ops.beam_reorder(now[2], slots, t.ctx_len, paged=[(kv, bt, 1)], out=mine)[1][0]
+            wait()
+        if written:
+            ops.rope_kv_write(qkv, None, t.positions, None, 0, nq, nkv, hd, t.slot_mappings[0], kv[0], kv[1], torch.bfloat16)
+            wait()
+        if form == "simt":
+            result.copy_(ops.attention_simt(q, kv[0], kv[1], bt, t.positions, t.seq_of_token, nq, nkv, hd, 0.1, None).view(S, -1))
+        elif form == "mma":
+            ops.attention_mma(q, kv[0], kv[1], bt, t.q_start, t.ctx_len, tiles, True, 1, nq, nkv, hd, 0.1, None, result)
+        else:
+            ops.attention_tma_decode(q, kv[0], kv[1], bt, t.q_start, t.ctx_len, tiles, 2, nq, nkv, hd, 0.1, None, result)
+
+    def take(i):
+        for a, b in zip(now, sets[i]):
+            a.copy_(b)
+        kv.copy_(kv0)
+        result.fill_(7.0)
+    want = []
+    for i in range(len(sets)):
+        take(i)
+        torch.cuda.synchronize()
+        turn(torch.cuda.synchronize)
+        torch.cuda.synchronize()
+        want.append(result.clone())
+    assert all(not torch.equal(a, b) for a, b in itertools.combinations(want, 2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        turn(lambda: None)
+    for step in (lambda: turn(lambda: None), graph.replay):
+        for i in list(range(len(sets))) * 5:
+            take(i)
+            step()
+            assert torch.equal(result, want[i]), i
+    ops.check_tcgen05_status()
