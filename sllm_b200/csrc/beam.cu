@@ -241,13 +241,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     return top;
   };
   // s: the sum of 2^(x log2 e - c) with c = m log2 e rounded; what the rounding left, `rest`, is taken out when m moves and at the end.  Where m log2 e has no place in
-  // float32 (an infinite m, rows at the type's ends), c is not a number and every batch goes the long way.
+  // float32 good to a fraction of one (an infinite m, logits of 10^6 and more, masked rows among them), c is not a number and every batch goes the long way.
   const float log2e = 1.4426950408889634f;
   float c = 0.f, rest = 0.f;
   auto add_up = [&](const float* x, float top) {
     if (top > m) {
       const float to = top * log2e;
-      const bool in = fabsf(to) < 1e38f;
+      const bool in = fabsf(to) < 1048576.f;           // (2^20: `rest` is 2^-5 at most)
       const float left = in ? fmaf(top, log2e, -to) : 0.f;
       if (m > -INFINITY) s *= exp2_fast((m - top) * log2e) * exp2_fast(left - rest);
       m = top;

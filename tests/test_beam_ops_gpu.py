@@ -98,6 +98,23 @@ def test_candidates_far_apart_scores_and_large_logits():
     _check_candidates(x, scores, 24)
 
 
+@pytest.mark.parametrize("V", [7, 1000, 20011])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_candidates_of_rows_of_huge_logits(V, dtype):
+    """Rows whose logits are all of a size where float32 has no fractions left (1e4 to the type's end, both signs; a mask of -1e30 everywhere): level ones, ones with a maximum of few, and with a beam of
+    ordinary logits beside them."""
+    dev = cuda_or_skip()
+    sizes = [s * m for m in (1e4, 5e5, 9e5, 2e6, 7e6, 1e8, 1e9, 1e10, 1e20, 1e30, 3e37, 1e38, 3e38) for s in (1, -1)]
+    g = torch.Generator(device=dev).manual_seed(V)
+    x = torch.empty(len(sizes), 3, V, device=dev)
+    for i, m in enumerate(sizes):
+        x[i, 0] = m
+        x[i, 1] = m * (1 + torch.rand(V, device=dev, generator=g) * 0.1)
+        x[i, 1, :: 3] = m if m > 0 else m * 1.1
+        x[i, 2] = torch.randn(V, device=dev, generator=g)
+    _check_candidates(x.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype).reshape(-1, V).contiguous(), -torch.rand(len(sizes), 3, device=dev, generator=g), 6)
+
+
 @pytest.mark.parametrize("V", [40, 3001, 50000])
 @pytest.mark.parametrize("keep", [1, 2, 3, 9])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
