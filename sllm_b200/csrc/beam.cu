@@ -7,10 +7,11 @@
 // logit, so a beam's own best are those of the largest logits, and no candidate of the search lies outside the `keep` best of its beam:
 //   beam_rows_kernel    a part of a row a block: the part's maximum, its sum of exponentials and its `keep` largest logits, from one pass over the logits;
 //   beam_merge_kernel   a block a search, a warp a beam: the beam's parts joined, then the beams.
-// Exponentials and a thread's sum of them are float32 (a few hundred terms, four sums a batch); the sums over threads and parts, the logarithm and s are float64, because continuations of
-// different beams are compared with each other (those of one beam by their logits alone).  s is rounded to float32 once, when it is stored.
-// Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 9.9 (0.4), 35 of 32,001 12.7 (0.7), 512 of 152,064 float32 62 (47.6) and
-// bfloat16 53 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
+// Exponentials and a batch's sum of them (16 terms) are float32; the sums over batches, threads and parts, the logarithm and s are of 48 bits and more, because continuations of different beams
+// are compared with each other (those of one beam by their logits alone).  Where two beams' lie closer than those float32 steps can tell, their sums are made again in float64 (see `beam_close`).
+// s is rounded to float32 once, when it is stored.
+// Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 10.8 (0.4), 35 of 32,001 13.9 (0.7), 512 of 152,064 float32 63 (47.6) and
+// bfloat16 54.5 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
 // through side by side.
 #include "common.cuh"
 
@@ -40,7 +41,26 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k)
   return (unsigned long long)hi << 32 | lo;
 }
 
-// a part of a row: the sum of exp(logit - max), and its largest logit
+// log2 e as the kernels multiply with it: 2^(x BEAM_LOG2E) is e^x but for 1.34e-8 |x| of it, and for 1.34e-8 |x - max| once the maximum is taken out in the same way.
+constexpr float BEAM_LOG2E = 1.4426950408889634f;
+
+// A sum of exponentials, Sum 2^(x BEAM_LOG2E), is held over 2^r.  r goes by the largest logit m alone: a whole number at m BEAM_LOG2E or just above it where float32 holds one to the unit
+// with room to spare (`beam_whole`; not a number elsewhere: infinite m, rows of 10^6 and more), so that sums of other maxima are brought to it by a change of exponent, exactly; m BEAM_LOG2E itself elsewhere.
+__device__ __forceinline__ float beam_whole(float m) {
+  const float to = m * BEAM_LOG2E;
+  return fabsf(to) < 4194304.f ? ceilf(to) : __uint_as_float(0x7fffffffu);
+}
+__device__ __forceinline__ double beam_reference(float m, float whole) { return whole == whole ? (double)whole : (double)m * (double)BEAM_LOG2E; }
+// 2^(r of m - r of top), m <= top; whole: theirs (minus infinity: nothing summed yet)
+__device__ __forceinline__ double beam_moved(float m, float whole, float top, float top_whole) {
+  if (whole <= top_whole) {
+    const float d = whole - top_whole;
+    return d > -1022.f ? __hiloint2double((1023 + (int)d) << 20, 0) : 0.0;
+  }
+  return exp2(beam_reference(m, whole) - beam_reference(top, top_whole));
+}
+
+// a part of a row: its sum of exponentials, and its largest logit
 struct BeamPart {
   double sum;
   float max;
@@ -191,8 +211,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // One part of one row: blockIdx.x = row * splits + part.  What bounds it: reading the logits once.  A batch is BEAM_VALUES logits a thread in 16-byte loads, all in flight
 // together, the next batch's under the arithmetic of this one.
-// An exponential is 2^(x log2 e - c) in one rounding of the exponent: off by about |x - m| + 4 units of 2^-24, of which the sum keeps the mean, |x - m| being at most ln V on
-// average under the softmax itself.
+// An exponential is 2^(x log2 e - c) in one rounding of the exponent, c a whole number; what it is off by: `beam_close`.
 // Of a batch only keys that reach the bound, a key that `keep` others are known to reach, can be among the best.  The first batch's bound comes from the threads' largest.  A run of
 // 6, then 36, ... batches is read without a barrier; a thread whose largest logit of a batch reaches the bound notes the batch (a vote of its warp, no atomics), and behind the run the noted
 // ones are read again (from L1 or L2), their keys join the list, and the list, cut to its `keep` largest, gives the next bound: of logits in no particular order five or six
@@ -214,7 +233,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
   if (threadIdx.x == 0) sh.n = 0;
   unsigned long long bound = (unsigned long long)(BEAM_MINUS_INFINITY + 1) << 32;
   float bound_logit = beam_value(BEAM_MINUS_INFINITY + 1);
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY, s = 0.f, s_low = 0.f;
   // the pieces of one thread's batch: first, first + BEAM_THREADS, ...
   auto fetch = [&](int first, bool all, uint4* raw) {
     if (all) {
@@ -240,40 +259,52 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     }
     return top;
   };
-  // s: the sum of 2^(x log2 e - c) with c = m log2 e rounded; what the rounding left, `rest`, is taken out when m moves and at the end.  Where m log2 e has no place in
-  // float32 good to a fraction of one (an infinite m, logits of 10^6 and more, masked rows among them), c is not a number and every batch goes the long way.
-  const float log2e = 1.4426950408889634f;
-  float c = 0.f, rest = 0.f;
+  // s + s_low: the sum of 2^(x log2 e - c), c the whole number of m; every batch's own sum is float32, what adding it to s rounds away goes into s_low (one float64 in their place: 512 rows
+  // of bfloat16 55.3 us for 54.5).  Where m has no such number c is none either and every batch goes the long way.
+  float c = -INFINITY;
+  auto split = [&](double sum) {
+    s = (float)sum;
+    s_low = (float)(sum - (double)s);
+  };
   auto add_up = [&](const float* x, float top) {
     if (top > m) {
-      const float to = top * log2e;
-      const bool in = fabsf(to) < 1048576.f;           // (2^20: `rest` is 2^-5 at most)
-      const float left = in ? fmaf(top, log2e, -to) : 0.f;
-      if (m > -INFINITY) s *= exp2_fast((m - top) * log2e) * exp2_fast(left - rest);
+      const float to = beam_whole(top);
+      if (c <= to) {
+        const float d = c - to, by = d > -126.f ? __uint_as_float((uint32_t)(127 + (int)d) << 23) : 0.f;
+        s *= by;
+        s_low *= by;
+      } else {
+        split(((double)s + (double)s_low) * beam_moved(m, c, top, to));
+      }
       m = top;
-      c = in ? to : __uint_as_float(0x7fffffffu);
-      rest = left;
+      c = to;
     }
     if (m > -INFINITY) {
-      const float2 by = make_float2(-c, -c), factor = make_float2(log2e, log2e);
+      const float2 by = make_float2(-c, -c), factor = make_float2(BEAM_LOG2E, BEAM_LOG2E);
       float2 p[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (int i = 0; i < BEAM_VALUES; i += 2) {
         const float2 t = fma2(make_float2(x[i], x[i + 1]), factor, by);
         p[(i >> 1) & 1] = add2(p[(i >> 1) & 1], make_float2(exp2_fast(t.x), exp2_fast(t.y)));
       }
-      float add = (p[0].x + p[0].y) + (p[1].x + p[1].y);
+      const float add = (p[0].x + p[0].y) + (p[1].x + p[1].y);
       // (asked of the bits: the compiler takes what the exponential's asm gives for numbers and leaves `add != add` out)
-      if ((__float_as_uint(add) & 0x7fffffffu) >= 0x7f800000u) {        // a logit that is none, which counts for nothing, or an infinite one, on which all of the mass lies
-        add = 0.f;
+      if ((__float_as_uint(add) & 0x7fffffffu) >= 0x7f800000u) {
+        // a logit that is none, which counts for nothing, or an m without a whole number: differences from it are exact where they count (those of an infinite m: all of the mass lies on the infinities)
+        const bool whole = (__float_as_uint(c) & 0x7fffffffu) < 0x7f800000u;
+        double sum = (double)s + (double)s_low;
 #pragma unroll
         for (int i = 0; i < BEAM_VALUES; ++i) {
-          if (x[i] == m) add += 1.f;
-          else if (x[i] < m && m < INFINITY) add += exp2_fast((x[i] - m) * log2e);
+          if (whole) sum += x[i] <= m ? (double)exp2_fast(fmaf(x[i], BEAM_LOG2E, -c)) : 0.0;
+          else if (x[i] == m) sum += 1.0;
+          else if (x[i] < m && m < INFINITY) sum += (double)exp2_fast((x[i] - m) * BEAM_LOG2E);
         }
-        add *= exp2_fast(rest);
+        split(sum);
+      } else {
+        const float sum = s + add, z = sum - s;
+        s_low += (s - (sum - z)) + (add - z);
+        s = sum;
       }
-      s += add;
     }
   };
   // a logit's key, 0 where it offers nothing; minus zero is zero
@@ -360,12 +391,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1024 / BEAM_THREADS) beam_rows_k
     }
   }
   pdl_launch_dependents();
-  // the part's maximum and sum: the threads' sums, brought to the same maximum, in 64 bits
+  // the part's maximum and sum: the threads' sums, brought to its maximum
   const float warp_top = warp_max(m);
   if (lane == 0) sh.red_m[warp] = warp_top;
   __syncthreads();
   const float all = warp_max(lane < BEAM_THREADS / 32 ? sh.red_m[lane] : -INFINITY);
-  double sum = m == all && m > -INFINITY ? (double)(s * exp2_fast(-rest)) : m > -INFINITY && all < INFINITY ? (double)(s * exp2_fast((m - all) * log2e - rest)) : 0.0;
+  double sum = (double)s + (double)s_low;
+  if (m != all) sum = m > -INFINITY && all < INFINITY ? sum * beam_moved(m, c, all, beam_whole(all)) : 0.0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sh.red_s[warp] = sum;
@@ -395,13 +427,90 @@ struct BeamHead {
   }
 };
 
-// Neighbours in the order that are two beams' and lie closer than this are told apart by the beams' sums in 64 bits throughout, which the block makes from the rows then (the parts' sums are good
-// to some 2^-25; a search of 8 beams meets this once in hundreds of calls, and a row of 152,064 takes it 60 us).
-constexpr double BEAM_CLOSE = 2.384185791015625e-7;           // 2^-22
+// Neighbours in the order that are two beams' and lie closer than `close` are told apart by the beams' sums in 64 bits throughout, which the block makes from the rows then.  `close` is twice what the
+// logarithm of a sum of the rows' kernel may be off by, in units of u = 2^-24, with means under the softmax itself, under which |t| of 2^t is log2 V + 1 at the most:
+//   the rounding of t = x log2 e - c         ln 2 (log2 V + 1)
+//   log2 e's own                             0.23 ln V
+//   the exponential (2^-22)                  4
+//   the float32 sum of a batch, 5 additions  5
+// together less than 0.86 log2 V + 9.8; the sums of batches, threads and parts change their reference exactly and lose nothing of that size.  (Of 152,064 logits: 24.9 u, 1.5e-6.)
+// Of 400 calls of 64 searches of 8 beams over 152,064 normal logits ten made sums again, two of them each, which took them 150 us more.
+static double beam_close(int V) { return 2.0 * (0.86 * log2((double)V) + 10.0) / 16777216.0; }
+
+// e^d, d <= 0, but for some (1 + |d| / 8) 2^-51 of it (d below -690: e^-690): d = n ln 2 / 64 + r, the Taylor polynomial of degree 5 of r (|r| <= ln 2 / 128 leaves 4e-17), 2^((n mod 64) / 64) from a table and the
+// rest of n into the exponent (Tang's table-driven method).  A sum of a row is bound by float64 instructions, half as many as without a table; and no branch, so that a thread's run side by side.
+constexpr int BEAM_POWERS = 64;
+__device__ __forceinline__ double exp_double(double d, const double* powers) {
+  const double e = fmax(d, -690.0);
+  const double shifted = fma(e, 64 / 0.69314718055994531, 6755399441055744.0);                // + 1.5 * 2^52: n in the low bits
+  const double n = shifted - 6755399441055744.0;
+  const double r = fma(n, -0.69314718055994531 / 64, e);
+  const double r2 = r * r;
+  const double tail = fma(fma(fma(r, 1.0 / 120, 1.0 / 24), r2, fma(r, 1.0 / 6, 0.5)), r2, r);      // e^r - 1
+  const int k = __double2loint(shifted);
+  const double p = powers[k & (BEAM_POWERS - 1)], v = fma(p, tail, p);
+  return __hiloint2double(__double2hiint(v) + ((k >> 6) << 20), __double2loint(v));
+}
+
+// What a beam's scores are made of: s + (x - top), less the logarithm of its sum.
+struct BeamRow {
+  float score, top;
+};
+__device__ __forceinline__ double beam_score(const BeamRow& r, float x, double lse) { return (double)r.score + ((x == r.top ? 0.0 : (double)x - (double)r.top) - lse); }
+
+// The beams in `close` of a search: their sums again, by the whole block, and their scores: 52 us a row of 152,064 that L2 holds.  (A function of its own, so that the join's instructions lie together;
+// within the join it took 8 rows of 4 beams 0.1 us more that made no sum again.)
+template <typename T>
+__device__ __noinline__ void beam_sums_again(const T* logits, int V, int B, int keep, unsigned close, const BeamRow* rows, const float* best_logit, unsigned long long* merged) {
+  __shared__ double red[BEAM_MAX], powers[BEAM_POWERS];
+  const int width = blockDim.x;
+  const T* search = logits + (size_t)blockIdx.x * B * V;
+  // the rows from HBM into L2, all at once: what a block's own loads have in flight would take as long again
+  for (unsigned left = close; left; left &= left - 1) {
+    const char* x_row = reinterpret_cast<const char*>(search + (size_t)(__ffs(left) - 1) * V);
+    for (size_t at = (size_t)threadIdx.x * 128; at < V * sizeof(T); at += (size_t)width * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(x_row + at));
+  }
+  for (int i = threadIdx.x; i < BEAM_POWERS; i += width) powers[i] = exp2((double)i / BEAM_POWERS);
+  __syncthreads();
+  for (unsigned left = close; left; left &= left - 1) {
+    const int c = __ffs(left) - 1;
+    const BeamRow row = rows[c];
+    if (!(row.top < INFINITY)) continue;            // (an infinite maximum: a count, which is exact)
+    const T* x_row = search + (size_t)c * V;
+    // eight logits of a thread a step, the next step's loaded under this one's exponentials
+    const double top = row.top;
+    double each[4] = {0.0, 0.0, 0.0, 0.0};
+    float next[8];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) next[u] = i0 + u * width < V ? to_f32(x_row[i0 + u * width]) : -INFINITY;
+    };
+    load(threadIdx.x);
+    for (int i0 = threadIdx.x; i0 < V; i0 += 8 * width) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = fmaxf(next[u], -INFINITY);                // (not a number: minus infinity)
+      load(i0 + 8 * width);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) each[u & 3] += exp_double((double)x[u] - top, powers);
+    }
+    double all = (each[0] + each[1]) + (each[2] + each[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = all;
+    __syncthreads();
+    double total = 0.0;
+    for (int w = 0; w < width / 32; ++w) total += red[w];
+    const double exact = fmax(log(total), 0.0);
+    for (int i = threadIdx.x; i < keep; i += width)
+      if (merged[c * keep + i] != 0) merged[c * keep + i] = order_double(beam_score(row, best_logit[c * keep + i], exact));
+    __syncthreads();
+  }
+}
 
 template <typename T>
-__global__ void beam_merge_kernel(const T* logits, int V, const float* scores, const BeamPart* parts, const unsigned long long* keys, int B, int keep, int splits, float* out_score,
-                                  int* out_parent, int* out_token) {
+__global__ void __launch_bounds__(32 * BEAM_MAX) beam_merge_kernel(const T* logits, int V, const float* scores, const BeamPart* parts, const unsigned long long* keys, int B, int keep, int splits, double close_by,
+                                  float* out_score, int* out_parent, int* out_token) {
   extern __shared__ __align__(16) unsigned char beam_smem[];
   unsigned long long* lists = reinterpret_cast<unsigned long long*>(beam_smem);        // [B][splits][keep]: a beam's parts
   unsigned long long* merged = lists + (size_t)B * splits * keep;                      // [B][keep]: a beam's keys joined, then its scores
@@ -409,54 +518,60 @@ __global__ void beam_merge_kernel(const T* logits, int V, const float* scores, c
   float* best_logit = reinterpret_cast<float*>(best_token + B * keep);                 // [B][keep]
   __shared__ int picked[BEAM_KEEP];                                                    // beam << 8 | place
   __shared__ unsigned close_s;
-  __shared__ double red[BEAM_MAX];
+  __shared__ BeamRow rows[BEAM_MAX];
   pdl_launch_dependents();
   pdl_wait();
   const int g = blockIdx.x, b = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const size_t row = (size_t)g * B + b;
-  const float score = scores[row];
-  unsigned long long *mine = lists + (size_t)b * splits * keep, *joined = merged + b * keep;
-  const unsigned long long* src = keys + row * splits * keep;
-  const BeamPart part = lane < splits ? parts[row * splits + lane] : BeamPart{0.0, -INFINITY};
+  if (b < B) {                                      // (warps behind the beams' are there for sums that are made again)
+    const size_t row = (size_t)g * B + b;
+    const float score = scores[row];
+    unsigned long long *mine = lists + (size_t)b * splits * keep, *joined = merged + b * keep;
+    const unsigned long long* src = keys + row * splits * keep;
+    const BeamPart part = lane < splits ? parts[row * splits + lane] : BeamPart{0.0, -INFINITY};
 #pragma unroll 4
-  for (int i = lane; i < splits * keep; i += 32) mine[i] = src[i];
-  const float top = warp_max(part.max);
-  double sum = 0.0;
-  if (part.max > -INFINITY && (top < INFINITY || part.max == top)) sum = part.max == top ? part.sum : part.sum * exp((double)part.max - (double)top);
-  if (splits > 1) {
+    for (int i = lane; i < splits * keep; i += 32) mine[i] = src[i];
+    const float top = warp_max(part.max), whole = beam_whole(top);
+    const BeamRow about = {score, top};
+    if (lane == 0) rows[b] = about;
+    double sum = 0.0;
+    if (part.max > -INFINITY && (top < INFINITY || part.max == top)) sum = part.max == top ? part.sum : part.sum * beam_moved(part.max, beam_whole(part.max), top, whole);
+    if (splits > 1) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  } else {
-    sum = __shfl_sync(0xffffffffu, sum, 0);
-  }
-  __syncwarp();
-  int found = 0;
-  if (splits > 1) {                                 // lane l walks the l-th part's list
-    BeamHead h(mine + lane * keep, lane < splits ? keep : 0);
-    for (; found < keep; ++found) {
-      const unsigned long long best = warp_max_key(h.head);
-      if (best == 0) break;
-      if (h.head == best) {
-        joined[found] = best;
-        h.pop();
-      }
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    } else {
+      sum = __shfl_sync(0xffffffffu, sum, 0);
     }
     __syncwarp();
-  } else {
-    joined = mine;
-    found = keep;
+    int found = 0;
+    if (splits > 1) {                               // lane l walks the l-th part's list
+      BeamHead h(mine + lane * keep, lane < splits ? keep : 0);
+      for (; found < keep; ++found) {
+        const unsigned long long best = warp_max_key(h.head);
+        if (best == 0) break;
+        if (h.head == best) {
+          joined[found] = best;
+          h.pop();
+        }
+      }
+      __syncwarp();
+    } else {
+      joined = mine;
+      found = keep;
+    }
+    const bool alive = score > -INFINITY && top > -INFINITY;
+    // (the maximum's own term is 1, so the logarithm is never below 0)
+    const double lse = fmax(whole == whole ? log(sum) + ((double)whole - (double)top * (double)BEAM_LOG2E) * 0.69314718055994531 : log(sum), 0.0);
+    for (int i = lane; i < keep; i += 32) {
+      const unsigned long long k = i < found && alive ? joined[i] : 0ull;
+      const float x = beam_value((uint32_t)(k >> 32));
+      const double v = beam_score(about, x, lse);
+      merged[b * keep + i] = k != 0 && v > -INFINITY ? order_double(v) : 0ull;
+      best_token[b * keep + i] = (int)~(uint32_t)k;
+      best_logit[b * keep + i] = x;
+    }
   }
-  const bool alive = score > -INFINITY && top > -INFINITY;
-  auto score_of = [&](float x, double lse) { return (double)score + ((x == top ? 0.0 : (double)x - (double)top) - lse); };
-  const double lse = log(sum);
-  for (int i = lane; i < keep; i += 32) {
-    const unsigned long long k = i < found && alive ? joined[i] : 0ull;
-    const float x = beam_value((uint32_t)(k >> 32));
-    const double v = score_of(x, lse);
-    merged[b * keep + i] = k != 0 && v > -INFINITY ? order_double(v) : 0ull;
-    best_token[b * keep + i] = (int)~(uint32_t)k;
-    best_logit[b * keep + i] = x;
-  }
+  // (a step of 64-bit scores beside it: what is far from 0 has few bits left behind the point)
+  auto close_to = [&](double v, double w) { return v - w < close_by + fabs(v) * 8.8817841970012523e-16; };       // 2^-50
   int n = 0;
   for (bool again = false;; again = true) {
     __syncthreads();
@@ -475,14 +590,14 @@ __global__ void beam_merge_kernel(const T* logits, int V, const float* scores, c
       __syncwarp();
       // the beams with one that is left out as close to the last that is not
       const double last = n > 0 ? double_of(merged[(picked[n - 1] >> 8) * keep + (picked[n - 1] & 255)]) : 0.0;
-      const unsigned behind = __ballot_sync(0xffffffffu, n > 0 && h.head != 0 && last - double_of(h.head) < BEAM_CLOSE);
+      const unsigned behind = __ballot_sync(0xffffffffu, n > 0 && h.head != 0 && close_to(last, double_of(h.head)));
       unsigned close = 0;
       for (int i = lane; i < n; i += 32) {
         const int a = picked[i] >> 8;
         const double v = double_of(merged[a * keep + (picked[i] & 255)]);
         if (i + 1 < n) {
           const int c = picked[i + 1] >> 8;
-          if (a != c && v - double_of(merged[c * keep + (picked[i + 1] & 255)]) < BEAM_CLOSE) close |= 1u << a | 1u << c;
+          if (a != c && close_to(v, double_of(merged[c * keep + (picked[i + 1] & 255)]))) close |= 1u << a | 1u << c;
         } else if (behind & ~(1u << a)) {
           close |= 1u << a | behind;
         }
@@ -493,33 +608,7 @@ __global__ void beam_merge_kernel(const T* logits, int V, const float* scores, c
     __syncthreads();
     const unsigned close = close_s;
     if (close == 0) break;
-    for (unsigned left = close; left; left &= left - 1) {
-      const int c = __ffs(left) - 1;
-      if (b == c && lane == 0) red[0] = (double)top;
-      __syncthreads();
-      const double c_top = red[0];
-      __syncthreads();
-      if (!(c_top < INFINITY)) continue;            // (an infinite maximum: a count, which is exact)
-      const T* x_row = logits + ((size_t)g * B + c) * V;
-      double all = 0.0;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < V; i += blockDim.x) {
-        const float x = to_f32(x_row[i]);
-        if (x > -INFINITY) all += exp((double)x - c_top);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-      if (lane == 0) red[b] = all;
-      __syncthreads();
-      if (b == c) {
-        double total = 0.0;
-        for (int w = 0; w < B; ++w) total += red[w];
-        const double exact = log(total);
-        for (int i = lane; i < keep; i += 32)
-          if (merged[c * keep + i] != 0) merged[c * keep + i] = order_double(score_of(best_logit[c * keep + i], exact));
-      }
-      __syncthreads();
-    }
+    beam_sums_again(logits, V, B, keep, close, rows, best_logit, merged);
   }
   if (b != 0) return;
   for (int i = lane; i < keep; i += 32) {
@@ -668,7 +757,8 @@ static bool beam_both(const T* logits, const float* scores, int G, int B, int V,
   if (!rows_limit.raise(beam_rows_kernel<T>, sizeof(BeamShared)) || !merge_limit.raise(beam_merge_kernel<T>, merge_smem)) return false;
   launch_kernel(beam_rows_kernel<T>, dim3((unsigned)(G * B * splits)), BEAM_THREADS, sizeof(BeamShared), stream, logits, V, keep, beam_log2_lanes(keep), splits,
                 ((V + N - 1) / N + splits - 1) / splits, parts, keys);
-  launch_kernel(beam_merge_kernel<T>, G, 32 * B, merge_smem, stream, logits, V, scores, (const BeamPart*)parts, (const unsigned long long*)keys, B, keep, splits, out_score, out_parent, out_token);
+  launch_kernel(beam_merge_kernel<T>, G, 32 * (B > 8 ? B : 8), merge_smem, stream, logits, V, scores, (const BeamPart*)parts, (const unsigned long long*)keys, B, keep, splits, beam_close(V),
+                out_score, out_parent, out_token);
   return true;
 }
 

@@ -2659,8 +2659,8 @@ def beam_candidates(logits: torch.Tensor, scores: torch.Tensor, keep: int):
     """The best continuations of ``G`` searches of ``B`` beams: ``logits`` (float32 or bfloat16 ``[G*B, V]``) of the beams' next
     tokens, ``scores`` (float32 ``[G, B]``) their cumulative log-probabilities.  Of all beams and tokens of a search the ``keep`` largest
     ``score + log_softmax(logits)``, in order: by that sum (compared in 64 bits), then the lower beam, the larger logit, the lower token.
-    (A beam's own tokens are ordered exactly.  The sum under a beam's logarithm is of float32 exponentials, good to some 1e-8 of itself; where neighbours in
-    the order are two beams' and lie closer than 2^-22, those beams' sums are made again in 64 bits.  Equal rows of equal score are equal in every bit.)
+    (A beam's own tokens are ordered exactly.  The sum under a beam's logarithm is of float32 exponentials, good to (0.86 log2 V + 10) 2^-24 of itself, 1.5e-6 for 152,064 logits;
+    where neighbours in the order are two beams' and lie closer than twice that, those beams' sums are made again in 64 bits.  Equal rows of equal score are equal in every bit.)
     Returns ``(scores float32, beams int32, tokens int32)``, each ``[G, keep]``.
 
     A beam whose score is minus infinity or not a number takes no part, nor does a logit that is; where there are fewer

@@ -134,6 +134,79 @@ def test_beams_whose_best_lie_next_to_each_other(V, keep, dtype):
     _check_candidates(logits, scores.contiguous(), keep)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", [8.0, 8.5, 9.0, 9.7, 10.3, 11.0, 11.6, 12.2, 13.0, "width 4", "width 6", "width 8", "rising"])
+@pytest.mark.parametrize("V", [152064, 152063])
+def test_beams_closer_than_sums_in_32_bits_tell_apart(V, kind, dtype):
+    """Whole rows (more than the SMs hold blocks) of two beams a search, whose best continuations lie 2^-24 to 2^-16 apart, either first: the order is the one of sums in 64 bits.  One logit above
+    equal ones (a number: by how much), where every rounding is the same one; rows of normal logits; rows that rise, whose maximum moves with every batch.  The other beam's row is one
+    logit, whose sum is exact, or normal too."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    G, B, keep = 160, 2, 2
+    g = torch.Generator(device=dev).manual_seed(V)
+    x = torch.full((G, B, V), -math.inf, device=dev)
+    if isinstance(kind, float):
+        x[:, 0] = 3.7 - kind
+        x[:, 0, 77] = 3.7
+    elif kind == "rising":
+        x[:, 0] = torch.arange(V, device=dev) * 1e-5
+        x[:, 0, V - 1] += 1.0
+    else:
+        x[:, 0] = torch.randn(G, V, device=dev, generator=g) * float(kind.split()[1])
+    x[:, 1, 5] = 0.25
+    if not isinstance(kind, float):
+        x[1::2, 1] = torch.randn(G // 2, V, device=dev, generator=g) * 4
+    x = x.to(dtype)
+    d = x.double()
+    lse = torch.logsumexp(d, 2)
+    best = d.amax(2) - lse
+    gap = torch.logspace(-24, -16, G // 4, base=2, device=dev, dtype=torch.float64).repeat_interleave(4) * torch.tensor([1.0, 1.0, -1.0, -1.0], device=dev, dtype=torch.float64).repeat(G // 4)
+    # the sum of the beam whose score has the finer steps is put beside the other's
+    scores = torch.empty(G, B, device=dev)
+    scores[:, 0] = (-0.06 - best[:, 0]).float()
+    scores[:, 1] = (scores[:, 0].double() + best[:, 0] + gap - best[:, 1]).float()
+    top, token = torch.sort(d, dim=2, descending=True, stable=True)
+    value = (scores.double()[:, :, None] + (top[:, :, :keep] - lse[:, :, None])).reshape(G, B * keep)
+    order = torch.sort(value, dim=1, descending=True, stable=True).indices[:, :keep]
+    token = torch.gather(token[:, :, :keep].reshape(G, B * keep), 1, order)
+    ahead = value.reshape(G, B, keep)[:, 0, 0] > value.reshape(G, B, keep)[:, 1, 0]
+    assert 0.3 < ahead.float().mean() < 0.7
+    s, p, t = ops.beam_candidates(x.reshape(G * B, V), scores, keep)
+    assert torch.equal(p.long(), order // keep) and torch.equal(t.long(), token), (int((p.long() != order // keep).sum()), int((t.long() != token).sum()))
+    want = torch.gather(value, 1, order).cpu().numpy()
+    assert (np.abs(s.cpu().numpy() - want) <= SCORE(want)).all()
+    # kept one: what is cut lies as close
+    s1, p1, t1 = ops.beam_candidates(x.reshape(G * B, V), scores, 1)
+    assert torch.equal(p1, p[:, :1]) and torch.equal(t1, t[:, :1]) and torch.equal(s1, s[:, :1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [700, 32001, 152064])
+def test_beams_closer_than_float32_numbers_are(V, dtype):
+    """A row of many logits beside one of a single logit, whose continuations' scores are near 0 and 2^-40 to 2^-24 apart: what tells them apart is the first row's sum.  Sums of at most 152,064
+    float64 exponentials, each right to 2^-51, added in some hundreds of steps a thread: within 2^-42 of the float64 reference, with room."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    G = 136
+    g = torch.Generator(device=dev).manual_seed(V + 1)
+    x = torch.full((G, 2, V), -math.inf, device=dev)
+    x[:, 0] = torch.randn(G, V, device=dev, generator=g) * torch.linspace(0, 9, G, device=dev)[:, None]
+    x[::3, 0, ::5], x[1::3, 0, 3::7] = -math.inf, math.nan
+    x[:, 1, 2] = 11.0
+    x = x.to(dtype)
+    d = torch.nan_to_num(x[:, 0].double(), nan=-math.inf)
+    best = d.amax(1) - torch.logsumexp(d, 1)
+    gap = torch.logspace(-40, -24, G // 2, base=2, device=dev, dtype=torch.float64).repeat_interleave(2) * torch.tensor([1.0, -1.0], device=dev, dtype=torch.float64).repeat(G // 2)
+    scores = torch.empty(G, 2, device=dev)
+    scores[:, 0] = -best.float()
+    scores[:, 1] = (scores[:, 0].double() + best + gap).float()
+    away = scores[:, 1].double() - (scores[:, 0].double() + best)
+    assert (away.abs() > 2.0 ** -42).all()
+    _, p, _ = ops.beam_candidates(x.reshape(2 * G, V), scores, 1)
+    assert torch.equal(p[:, 0] == 1, away > 0), torch.nonzero((p[:, 0] == 1) != (away > 0)).tolist()
+
+
 @pytest.mark.parametrize("keep", [1, 7, 64, 128])
 @pytest.mark.parametrize("kind", ["rising", "falling", "level", "steps"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
