@@ -13,6 +13,8 @@
 // Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 10.8 (0.4), 35 of 32,001 13.9 (0.7), 512 of 152,064 float32 63 (47.6) and
 // bfloat16 54.5 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
 // through side by side.
+#include <float.h>
+
 #include "common.cuh"
 
 namespace sllm {
@@ -681,7 +683,7 @@ __global__ void __launch_bounds__(32) beam_advance_kernel(const float* c_score, 
       cs[j] = in ? c_score[(size_t)g * keep + r] : -INFINITY;
       cp[j] = in ? c_parent[(size_t)g * keep + r] : -1;
       ct[j] = in ? c_token[(size_t)g * keep + r] : -1;
-      norm[j] = (float)((double)cs[j] / length);
+      norm[j] = fmaxf((float)((double)cs[j] / length), cs[j] > -INFINITY ? -FLT_MAX : -INFINITY);         // (a finite score's: minus infinity is an empty place)
       bool stop = false;
       for (int k = 0; k < stops; ++k) stop |= stop_ids[k] == ct[j];
       const bool there = cs[j] > -INFINITY;

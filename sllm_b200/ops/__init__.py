@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from collections import namedtuple
 from contextlib import suppress
@@ -2702,7 +2703,8 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
 
     Returns a `BeamStep`: ``scores``, ``parents`` and ``tokens`` ``[G, beams]`` of the next beams (fewer than ``beams``: minus infinity, -1,
     0; a search that is over: minus infinity, each beam its own parent, 0), the new ``lengths``, ``done`` and ``pool``; a search that was over before keeps
-    its pool and length.  ``out``: a `BeamStep` of tensors to write, the inputs' own among them.  At most 32 beams, a pool of 32 and 128 candidates."""
+    its pool and length.  (``max_new ** length_penalty`` is within 2^-64 and 2^64, so that float32 tells finished scores apart; what is below float32's lowest number is that.)
+    ``out``: a `BeamStep` of tensors to write, the inputs' own among them.  At most 32 beams, a pool of 32 and 128 candidates."""
     if out is None:
         out = _NO_STEP
         _here("beam_advance", scores, parents, tokens, *pool, lengths, done, stop_ids)
@@ -2714,6 +2716,8 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     if not 1 <= keep <= MAX_CANDIDATES or not 1 <= beams <= MAX_BEAMS or not 1 <= W <= MAX_BEAMS or not 1 <= max_new < 1 << 30 or not abs(power) < 64:
         raise KernelError(f"beam_advance: {keep} candidates (1 to {MAX_CANDIDATES}), {beams} beams and a pool of {W} (1 to {MAX_BEAMS}), "
                           f"max_new {max_new}, length penalty {power}")
+    if abs(power) * math.log2(max_new) > 64:
+        raise KernelError(f"beam_advance: {max_new} ** {power} leaves the range in which float32 keeps finished scores apart (2^-64 to 2^64)")
     i32, f32, of, ow, each = torch.int32, torch.float32, scores.shape, pool.scores.shape, (G,)
     if not (scores.dtype is f32 and pool.scores.dtype is f32 and ow[0] == G and parents.shape == of and tokens.shape == of and pool.lengths.shape == ow and pool.parents.shape == ow and
             pool.tokens.shape == ow and lengths.shape == each and done.shape == each and

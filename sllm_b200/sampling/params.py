@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 
@@ -57,6 +58,8 @@ class BeamParams:
             raise ValueError("max_new must be >= 1")
         if not abs(self.length_penalty) < 64:
             raise ValueError("length_penalty must be between -64 and 64")
+        if abs(self.length_penalty) * math.log2(self.max_new) > 64:
+            raise ValueError(f"length_penalty {self.length_penalty} at {self.max_new} tokens: the scores of finished continuations would leave float32 (max_new ** length_penalty is within 2^-64 and 2^64)")
         if self.keep > 128:
             raise ValueError(f"{self.beams} beams with {len(self.stop_ids)} stop ids need {self.keep} candidates a step, 128 at most")
 

@@ -294,6 +294,22 @@ def test_advance(B, K, stops, power):
                 assert got.pool[i][g].tolist() == [e[i] for e in after]
 
 
+@pytest.mark.parametrize("power,max_new", [(-6.4, 1000), (6.4, 1000), (-16.0, 16), (63.0, 2), (-2.1, 1 << 29), (-1.0, 100)])
+def test_advance_at_the_ends_of_float32(power, max_new):
+    """Penalties up to the largest that are taken, scores from one step of float32 below 0 to its lowest number: nothing that finishes is lost, and the pool is in the order of the scores."""
+    import sllm_b200.ops as ops
+    dev = cuda_or_skip()
+    low = float(torch.finfo(torch.float32).min)
+    s = torch.tensor([[-(2.0 ** -24), -1.0, -50.0, -1e12, -1e30, low]], device=dev)
+    got = ops.beam_advance(s, _i32([[0, 1, 2, 3, 4, 5]], dev), _i32([[9, 8, 7, 6, 5, 4]], dev), ops.beam_pool(1, 6, dev), _i32([max_new - 1], dev), _i32([0], dev), beams=6, max_new=max_new,
+                           length_penalty=power)
+    exact = s[0].double().cpu().numpy() / np.float64(max_new) ** power
+    want = np.maximum(exact, np.float64(low))
+    pool = got.pool.scores[0].cpu().numpy().astype(np.float64)
+    assert (np.abs(pool - want) <= 2.0 ** -24 * np.abs(want)).all(), (pool, want)
+    assert got.pool.tokens[0].tolist() == [9, 8, 7, 6, 5, 4] and got.pool.lengths[0].tolist() == [max_new] * 6 and got.done.tolist() == [1]
+
+
 def _reorder_case(rng, G, B, lens, stride_of, kinds, dev):
     """Pages of every search: shared whole ones, then one a beam and column; states of several types."""
     paged = []

@@ -363,6 +363,24 @@ def test_refusals_of_the_operators(unlaunched):
         assert len(calls) == len(good), i
 
 
+def test_penalties_that_leave_float32_are_refused(unlaunched):
+    """At 16 tokens and -33 a finished continuation's score was minus infinity, which is an empty place of the pool."""
+    ops, calls = unlaunched
+    pool = ops.BeamPool(torch.zeros(2, 3), _i(2, 3), _i(2, 3), _i(2, 3))
+    for power, max_new, taken in ((-33.0, 16, False), (33.0, 16, False), (16.0, 16, True), (-16.0, 16, True), (16.1, 16, False), (63.0, 2, True), (63.9, 1, True), (-3.0, 1 << 29, False), (-2.1, 1 << 29, True)):
+        n = len(calls)
+        kw = dict(max_new=max_new, length_penalty=power)
+        if taken:
+            ops.beam_advance(torch.zeros(2, 4), _i(2, 4), _i(2, 4), pool, _i(2), _i(2), beams=3, **kw)
+            assert len(calls) == n + 1 and BeamParams(**kw).length_penalty == power
+        else:
+            with pytest.raises(ops.KernelError, match="float32"):
+                ops.beam_advance(torch.zeros(2, 4), _i(2, 4), _i(2, 4), pool, _i(2), _i(2), beams=3, **kw)
+            with pytest.raises(ValueError, match="float32"):
+                BeamParams(**kw)
+            assert len(calls) == n
+
+
 def test_the_operators_take_no_cpu_tensors_and_no_strided_ones():
     import sllm_b200.ops as ops
     with pytest.raises(ops.KernelError, match="CUDA device"):
