@@ -2651,6 +2651,21 @@ def _typed(what: str, dtype, shape, *tensors) -> None:
             raise KernelError(f"{what}: {t.dtype} {tuple(t.shape)}, not {dtype} {shape}")
 
 
+def _apart(what: str, written, read, own=()) -> None:
+    """No tensor of ``written`` shares memory with another, or with one of ``read``.  ``own``: pairs (written, read) of which the one may be the whole other."""
+    same = {(id(w), id(r)) for w, r in own if w is not None and w.data_ptr() == r.data_ptr() and w.shape == r.shape}
+    gone = {r for _, r in same}
+    spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), True) for t in written if t is not None and t.numel()] +
+                   [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), False) for t in read if t is not None and t.numel() and id(t) not in gone])
+    end = end_written = 0
+    for first, last, is_written in spans:
+        if first < (end if is_written else end_written):
+            raise KernelError(f"{what}: what is written cannot be what is read, nor lie over another result")
+        end = max(end, last)
+        if is_written:
+            end_written = max(end_written, last)
+
+
 @functools.lru_cache(maxsize=4096)
 def _beam_splits(device: int, G: int, B: int, V: int) -> int:
     return lib().sllm_beam_splits(G, B, V)
@@ -2704,7 +2719,7 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
     Returns a `BeamStep`: ``scores``, ``parents`` and ``tokens`` ``[G, beams]`` of the next beams (fewer than ``beams``: minus infinity, -1,
     0; a search that is over: minus infinity, each beam its own parent, 0), the new ``lengths``, ``done`` and ``pool``; a search that was over before keeps
     its pool and length.  (``max_new ** length_penalty`` is within 2^-64 and 2^64, so that float32 tells finished scores apart; what is below float32's lowest number is that.)
-    ``out``: a `BeamStep` of tensors to write, the inputs' own among them.  At most 32 beams, a pool of 32 and 128 candidates."""
+    ``out``: a `BeamStep` of tensors to write; each may be the input of its kind (``scores``, ``parents`` and ``tokens`` where ``keep`` is ``beams``), none may lie over another input or result.  At most 32 beams, a pool of 32 and 128 candidates."""
     if out is None:
         out = _NO_STEP
         _here("beam_advance", scores, parents, tokens, *pool, lengths, done, stop_ids)
@@ -2745,6 +2760,9 @@ def beam_advance(scores, parents, tokens, pool: BeamPool, lengths, done, *, beam
         _typed("beam_advance: out.lengths and done", i32, (G,), res.lengths, res.done)
         _typed("beam_advance: out.pool", f32, (G, W), res.pool.scores)
         _typed("beam_advance: out.pool", i32, (G, W), *res.pool[1:])
+        # (a search's block reads its rows before it writes them: a result may be the input of its kind, whole, and no other part of one)
+        _apart("beam_advance", (*res[:5], *res.pool), (scores, parents, tokens, *pool, lengths, done, stop_ids),
+               own=zip((*res[:5], *res.pool), (scores, parents, tokens, lengths, done, *pool)))
     if G:
         p, q = pool, res.pool
         call("sllm_beam_advance", scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), G, keep, beams, W, p[0].data_ptr(), p[1].data_ptr(), p[2].data_ptr(), p[3].data_ptr(),
@@ -2778,7 +2796,7 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
     if new_slots is None:
         new_slots = torch.empty_like(slots)
     _typed("beam_reorder: new slots", torch.int32, (G * B,), new_slots)
-    about, made, read = [], [], {slots.data_ptr(), parents.data_ptr(), lens.data_ptr()}
+    about, made = [], []
     for (storage, table, stride), new in zip(paged, tables):
         if storage.dim() < 4 or stride < 1 or storage.element_size() < 2:
             raise KernelError(f"beam_reorder: a cache {storage.dtype} {tuple(storage.shape)}, an entry per {stride} tokens")
@@ -2789,7 +2807,6 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
             new = torch.empty_like(table)
         _typed("beam_reorder: a new block table", torch.int32, tuple(table.shape), new)
         made.append(new)
-        read.add(table.data_ptr())
         pages, heads, page_size, dim = storage.shape[-4:]
         if storage.numel() == 0:
             raise KernelError("beam_reorder: a cache without pages")
@@ -2798,8 +2815,8 @@ def beam_reorder(parents, slots, lens, *, states=(), paged=(), out=None):
             about += (storage.data_ptr(), table.data_ptr(), new.data_ptr(), dim * storage.element_size(), outer, heads, pages, page_size, stride, table.shape[1])
     if G == 0:
         return new_slots, made
-    if any(t.numel() and t.data_ptr() in read for t in (new_slots, *made)):
-        raise KernelError("beam_reorder: what is written cannot be what is read")
+    if out is not None:
+        _apart("beam_reorder", (new_slots, *made), (parents, slots, lens, *states, *(x for p in paged for x in p[:2])))
     rows = []
     for t in states:
         if t.dim() < 1:
@@ -2854,7 +2871,8 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
     columns = [t.shape[1] if c is None else int(c) for t, c in zip(page_tables, columns)]
     if n and min(columns) < 0:
         raise KernelError(f"step_tables: {columns} columns")
-    if out is None:
+    given = out is not None
+    if not given:
         dev = q_lens.device
         q_start, ctx_len, positions, seq_of_token, *maps = torch.empty(2 * S + 1 + (2 + n) * T, dtype=torch.int32, device=dev).split_with_sizes([S + 1, S] + [T] * (2 + n))
         out = StepTables(q_start, ctx_len, positions, seq_of_token, tuple([torch.empty(S, c, dtype=torch.int32, device=dev) for c in columns]), tuple(maps))
@@ -2866,9 +2884,10 @@ def step_tables(q_lens, have, page_tables, *, page_size: int, num_tokens: int, s
             raise KernelError("step_tables: out has other groups")
         for t, c in zip(out.block_tables, columns):
             _typed("step_tables: out.block_tables", torch.int32, (S, c), t)
-        read = {t.data_ptr() for t in (q_lens, have, rows, *page_tables, *free) if t is not None and t.numel()}
-        if any(t.numel() and t.data_ptr() in read for t in (*out[:4], *out.block_tables, *out.slot_mappings)):
-            raise KernelError("step_tables: what is written cannot be what is read")
+    grown = [t for t, f in zip(page_tables, free) if f is not None]
+    if given or grown:
+        kept = [t for t, f in zip(page_tables, free) if f is None]
+        _apart("step_tables", ((*out[:4], *out.block_tables, *out.slot_mappings) if given else ()) + tuple(grown), (q_lens, have, rows, *kept, *free))
     about = []
     for t, f, c, st, b, m in zip(page_tables, free, columns, strides, out.block_tables, out.slot_mappings):
         # (an empty list of free pages is still a list: its pointer only has to be one)

@@ -363,6 +363,53 @@ def test_refusals_of_the_operators(unlaunched):
         assert len(calls) == len(good), i
 
 
+def test_results_that_lie_over_what_is_read_are_refused(unlaunched):
+    """Blocks of other searches, or other threads, read there while one writes."""
+    ops, calls = unlaunched
+    G, B, keep, W = 2, 3, 6, 3
+    flat, ints = torch.zeros(400), _i(4000)
+    s, p, t, lengths, done, stops = flat[:G * keep].view(G, keep), ints[:12].view(G, keep), ints[12:24].view(G, keep), ints[30:32], ints[32:34], ints[40:42]
+    pool = ops.BeamPool(flat[20:26].view(G, W), *(ints[50 + 6 * i:56 + 6 * i].view(G, W) for i in range(3)))
+    none = ops.BeamStep(*(None,) * 5, ops.BeamPool(*(None,) * 4))
+
+    def advance(s=s, p=p, t=t, **out):
+        held = {k: out.pop(k) for k in ("pool",) if k in out}
+        ops.beam_advance(s, p, t, pool, lengths, done, beams=B, max_new=9, stop_ids=stops, out=none._replace(**out, **held))
+    # a result that is the input of its kind; candidates as many as beams among them
+    s3, p3, t3 = flat[100:106].view(G, B), ints[100:106].view(G, B), ints[106:112].view(G, B)
+    good = [lambda: advance(pool=pool, lengths=lengths, done=done), lambda: advance(s=s3, p=p3, t=t3, scores=s3, parents=p3, tokens=t3), lambda: advance(scores=flat[12:18].view(G, B)),
+            lambda: advance(pool=pool._replace(tokens=None))]
+    bad = [lambda: advance(scores=flat[:6].view(G, B)), lambda: advance(scores=flat[8:14].view(G, B)), lambda: advance(parents=ints[:6].view(G, B)), lambda: advance(tokens=ints[18:24].view(G, B)),
+           lambda: advance(lengths=done), lambda: advance(lengths=done, done=lengths), lambda: advance(done=stops), lambda: advance(parents=ints[200:206].view(G, B), tokens=ints[203:209].view(G, B)),
+           lambda: advance(pool=pool._replace(tokens=pool.parents)), lambda: advance(pool=pool._replace(parents=pool.tokens, tokens=pool.parents)), lambda: advance(pool=pool._replace(scores=flat[23:29].view(G, W))),
+           lambda: advance(s=s3, p=p3, t=t3, parents=t3), lambda: advance(s=s3, p=p3, t=t3, scores=flat[101:107].view(G, B))]
+    table, other, slots, lens, kv = ints[300:312].view(6, 2), ints[400:412].view(6, 2), ints[320:326], ints[330:332], torch.zeros(2, 5, 1, 16, 8)
+
+    def reorder(new_slots, new_table, more=()):
+        ops.beam_reorder(ints[340:346].view(G, B), slots, lens, paged=((kv, table, 1), *(((kv, other, 1),) if more else ())), out=(new_slots, [new_table, *more]))
+    good += [lambda: reorder(ints[500:506], ints[510:522].view(6, 2)), lambda: reorder(ints[500:506], ints[510:522].view(6, 2), (ints[522:534].view(6, 2),))]
+    bad += [lambda: reorder(ints[322:328], ints[510:522].view(6, 2)), lambda: reorder(ints[500:506], ints[306:318].view(6, 2)), lambda: reorder(ints[500:506], ints[500:512].view(6, 2)),
+            lambda: reorder(ints[341:347], ints[510:522].view(6, 2)), lambda: reorder(ints[327:333], ints[510:522].view(6, 2)), lambda: reorder(ints[500:506], ints[510:522].view(6, 2), (ints[410:422].view(6, 2),)),
+            lambda: reorder(ints[500:506], ints[510:522].view(6, 2), (ints[521:533].view(6, 2),))]
+
+    def tables(pages=(ints[600:608].view(4, 2),), free=None, q=ints[620:623], have=ints[630:633], slot=ints[1100:1103], **out):
+        made = ops.StepTables(ints[1000:1004], ints[1010:1013], ints[1020:1023], ints[1030:1033], tuple(ints[1040 + 10 * i:1046 + 10 * i].view(3, 2) for i in range(len(pages))),
+                              (slot, *(ints[1110 + 10 * i:1113 + 10 * i] for i in range(len(pages) - 1))))
+        ops.step_tables(q, have, pages, page_size=16, num_tokens=3, free=free, out=made._replace(**out))
+    two = (ints[600:608].view(4, 2), ints[610:618].view(4, 2))
+    good += [tables, lambda: tables(pages=two, free=[ints[700:705], None]), lambda: tables(pages=(two[0], two[0])), lambda: tables(pages=two, free=[ints[700:705], ints[700:705]])]
+    bad += [lambda: tables(ctx_len=ints[630:633]), lambda: tables(ctx_len=ints[628:631]), lambda: tables(q_start=ints[619:623]), lambda: tables(positions=ints[1030:1033]), lambda: tables(slot=ints[607:610]),
+            lambda: tables(pages=(two[0], two[0]), free=[ints[700:705], ints[710:715]]), lambda: tables(pages=(two[0], ints[604:612].view(4, 2)), free=[ints[700:705], None]),
+            lambda: tables(free=[ints[605:609]]), lambda: tables(free=[ints[700:705]], slot=ints[704:707])]
+    for i, g in enumerate(good):
+        g()
+        assert len(calls) == i + 1, i
+    for i, b in enumerate(bad):
+        with pytest.raises(ops.KernelError, match="cannot be what is read"):
+            b()
+        assert len(calls) == len(good), i
+
+
 def test_penalties_that_leave_float32_are_refused(unlaunched):
     """At 16 tokens and -33 a finished continuation's score was minus infinity, which is an empty place of the pool."""
     ops, calls = unlaunched
