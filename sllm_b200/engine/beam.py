@@ -139,7 +139,7 @@ class BeamSearch:
         self._calls = 0
 
     def search(self, prompts, params: BeamParams | None = None) -> list:
-        """Per prompt (a list of token ids), its `BeamResult`s, best first.  Prompts that fit side by side run side by side."""
+        """Per prompt (a list of token ids), its `BeamResult`s, best first.  Prompts that fit side by side run side by side; where one fits in no case, none runs."""
         params = replace(params or BeamParams())         # (checked again, and ours: the kept graphs are made for it)
         prompts = [[int(t) for t in p] for p in prompts]
         eng = self.engine
@@ -152,6 +152,8 @@ class BeamSearch:
                 raise ValueError("a prompt's token id is outside the vocabulary")
         if any(not 0 <= s < eng.vocab_size for s in params.stop_ids):
             raise ValueError("a stop id is outside the vocabulary")
+        for p in prompts:                         # each by itself fits what is free, before any of them runs (it all comes back between them)
+            self._fitting([p], params)
         results, at = [], 0
         while at < len(prompts):
             n = self._fitting(prompts[at:], params)

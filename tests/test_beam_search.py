@@ -241,6 +241,18 @@ def test_refused_searches(tmp_path, beam_cpu_ops):
     assert BeamParams(beams=3).results == 3 and BeamParams(beams=3, stop_ids=(4, 4, 2)).keep == 9
 
 
+def test_a_prompt_that_cannot_fit_is_found_before_the_others_run(tmp_path, beam_cpu_ops):
+    d, page, vocab, _ = _model(tmp_path, "qwen2")
+    llm = _llm(d, page, "cpu", 4, 8)
+    fits, never = [1, 2, 3], list(range(100))
+    steps = llm.engine.steps_run
+    for prompts in ([fits, never], [fits, fits, never, fits], [never, fits]):
+        with pytest.raises(OutOfPages, match="over 100"):
+            llm.beam_search(prompts, BeamParams(beams=4, max_new=20))
+        assert llm.engine.steps_run == steps and not llm.engine.cache.requests
+    assert len(llm.beam_search([fits, fits], BeamParams(beams=4, max_new=2))) == 2
+
+
 def test_a_search_that_fails_gives_everything_back(tmp_path, beam_cpu_ops, monkeypatch):
     d, page, _, _ = _model(tmp_path, "qwen2")
     llm = _llm(d, page, "cpu", 4, 40)
