@@ -9,7 +9,7 @@ and its dev command line (serving/cli.py:18-23: ``--temperature``, ``--top-p``,
 (serving/main.py:250-259).  ``serve`` (the HTTP server), ``--cpu`` and
 ``--placement um`` (host-memory decode) name things this engine does not have and
 are refused with a plain sentence.  Added here: ``--prompt-ids``, ``--dtype``,
-``--random-weights SEED``, ``--beams`` and ``--length-penalty`` (a beam search in sampling's place).
+``--random-weights SEED``, ``--stop-ids``, ``--beams`` and ``--length-penalty`` (a beam search in sampling's place).
 """
 
 from __future__ import annotations
@@ -98,7 +98,8 @@ def main(argv=None) -> int:
     ap.add_argument("--seed", type=int, default=None)
     ap.add_argument("--repetition-penalty", type=float, default=None)
     ap.add_argument("--beams", type=int, default=None, metavar="N", help="beam search with N beams; the best continuation is printed")
-    ap.add_argument("--length-penalty", type=float, default=1.0, help="of a beam search: scores are over tokens ** this")
+    ap.add_argument("--length-penalty", type=float, default=1.0, help="of a beam search: scores are over tokens ** this (continuations of different lengths end with one of --stop-ids)")
+    ap.add_argument("--stop-ids", default=None, help="comma-separated token ids; one of them ends a continuation and is not part of it")
     ap.add_argument("--dtype", choices=("bfloat16", "float32", "bf16", "fp32"), default=None)
     ap.add_argument("--random-weights", type=int, default=None, metavar="SEED",
                     help="write a random model folder from the recipe's geometry and run it")
@@ -119,6 +120,10 @@ def main(argv=None) -> int:
         raise SystemExit("sllm: this engine has no CPU or host-memory path; it runs on one B200")
     if args.beams is not None and (args.temperature > 0 or args.top_k is not None or args.top_p is not None or args.repetition_penalty is not None):
         raise SystemExit("sllm: --beams searches; it takes no --temperature, --top-k, --top-p or --repetition-penalty")
+    try:
+        stop_ids = tuple(int(x) for x in args.stop_ids.replace(" ", "").split(",") if x) if args.stop_ids else ()
+    except ValueError:
+        raise SystemExit(f"sllm: --stop-ids {args.stop_ids}: not a list of token ids") from None
     if args.nodes not in (None, 1):
         raise SystemExit(f"sllm: --tp {args.nodes}: this engine runs on one GPU")
     try:
@@ -154,7 +159,7 @@ def main(argv=None) -> int:
         from ..engine.llm import LLM
         from ..sampling import BeamParams, SamplingParams
         try:
-            beams = BeamParams(beams=args.beams, max_new=settings["max_new"], length_penalty=args.length_penalty) if args.beams is not None else None
+            beams = BeamParams(beams=args.beams, max_new=settings["max_new"], length_penalty=args.length_penalty, stop_ids=stop_ids) if args.beams is not None else None
         except ValueError as e:
             raise SystemExit(f"sllm: {e}") from None
         llm = LLM(model_dir, dtype=dtype, block_size=settings["block_size"], max_num_seqs=settings["max_num_seqs"],
@@ -162,6 +167,8 @@ def main(argv=None) -> int:
                   kv_utilization=recipe.kv_utilization, kv_bytes=recipe.kv_device_bytes,
                   progress=lambda d, t: log("INFO", f"load: {d}/{t} tensors"))
         vocab = llm.model.plan.vocab_size
+        if any(not 0 <= s < vocab for s in stop_ids):
+            raise SystemExit(f"sllm: --stop-ids {args.stop_ids}: the vocabulary has {vocab} tokens")
         tok = None
         if args.prompt_ids:
             prompts = [[int(x) for x in args.prompt_ids.replace(" ", "").split(",") if x]]
@@ -172,7 +179,7 @@ def main(argv=None) -> int:
             texts = args.batch or [args.chat if args.chat is not None else (args.prompt if args.prompt is not None else "hello")]
             prompts = [tok.encode(t) for t in texts]
         params = SamplingParams(max_new=settings["max_new"], temperature=args.temperature, top_k=args.top_k,
-                                top_p=args.top_p, seed=args.seed, repetition_penalty=args.repetition_penalty)
+                                top_p=args.top_p, seed=args.seed, repetition_penalty=args.repetition_penalty, stop_ids=stop_ids)
         import time
         t0 = time.perf_counter()
         if beams is not None:

@@ -477,3 +477,28 @@ def test_beams_of_the_command_line(beam_cpu_ops, capsys, monkeypatch):
         with pytest.raises(SystemExit) as e:
             cli.main(common + more)
         assert word in str(e.value)
+
+
+def test_stop_ids_and_the_length_penalty_of_the_command_line(beam_cpu_ops, capsys, monkeypatch):
+    """A continuation that stops at once has one log-probability, one of four tokens four of about the same: by their sums the first is the better, by their means of a high power the second."""
+    import sllm_b200.engine.llm as llm_mod
+    from sllm_b200.serving import main as cli
+    real = llm_mod.LLM
+    monkeypatch.setattr(llm_mod, "LLM", lambda model_dir, **kw: real(model_dir, **{**kw, "device": "cpu", "num_pages": 64}))
+    common = ["tiny-qwen2", "--mode", "run", "--random-weights", "3", "--prompt-ids", "5,6,7", "--max-new", "4", "--dtype", "float32", "--log-level", "ERROR"]
+
+    def ids(*more):
+        assert cli.main(common + list(more)) == 0
+        return [int(x) for x in capsys.readouterr().out.strip().split(",") if x]
+    greedy = ids()
+    assert len(greedy) == 4
+    stop = ["--stop-ids", str(greedy[0])]
+    assert ids(*stop) == []
+    assert ids("--beams", "3", "--length-penalty", "0", *stop) == []
+    found = ids("--beams", "3", "--length-penalty", "5", *stop)
+    assert len(found) == 4 and greedy[0] not in found
+    for bad, word in (("1,x", "token ids"), ("9999999", "vocabulary"), ("-1", "vocabulary")):
+        with pytest.raises(SystemExit, match=word):
+            cli.main(common + ["--stop-ids=" + bad])
+    with pytest.raises(SystemExit, match="float32"):
+        cli.main(common + ["--beams", "3", "--length-penalty", "40"])
