@@ -163,6 +163,49 @@ def test_rows_of_a_search_that_is_over_at_once_hold_its_prompt(tmp_path, arch, d
     llm.engine.cache.check()
 
 
+@pytest.mark.parametrize("arch", ARCHITECTURES)
+def test_more_beams_than_first_tokens(tmp_path, arch, dev, monkeypatch):
+    """Two tokens above minus infinity behind the prompt: the other beams idle for a step, over pages and states that hold the prompt, and are taken by the second step's continuations."""
+    import sllm_b200.ops as ops
+    monkeypatch.setenv("SLLM_POISON_FREED_PAGES", "1")
+    d, page, vocab, logits_of = _model(tmp_path, arch)
+    rng = np.random.default_rng(13)
+    prompts = [rng.integers(0, vocab, n).tolist() for n in (page + 3, 2 * page)]
+    two = [np.argsort(-logits_of(p))[3:5].tolist() for p in prompts]
+    candidates, seen = ops.beam_candidates, []
+
+    def beam_candidates(logits, scores, keep):
+        if scores.shape[1] == 1:
+            masked = torch.full_like(logits, -float("inf"))
+            for g, t in enumerate(two):
+                masked[g, t] = logits[g, t]
+            logits = masked
+        else:
+            seen.append(bool(torch.isnan(logits).any()))
+        return candidates(logits, scores, keep)
+    monkeypatch.setattr(ops, "beam_candidates", beam_candidates)
+
+    def masked_logits_of(g):
+        def of(ids):
+            logits = logits_of(ids)
+            if len(ids) > len(prompts[g]):
+                return logits
+            masked = np.full_like(logits, -np.inf)
+            masked[two[g]] = logits[two[g]]
+            return masked
+        return of
+    params = BeamParams(beams=5, max_new=4)
+    got = _llm(d, page, dev, 10, 400, cuda_graphs=False).beam_search(prompts, params)
+    assert seen and not any(seen)
+    for g, p in enumerate(prompts):
+        want = plain.search(masked_logits_of(g), p, beams=5, max_new=4)
+        assert {r.ids[0] for r in got[g]} <= set(two[g])
+        assert len(got[g]) == len(want) == 5
+        for r, (ids, norm, reason) in zip(got[g], want):
+            slack = 12e-4 * 4 * (1 + max(np.abs(logits_of(p + r.ids[:i])).max() for i in range(4)))
+            assert abs(r.score - norm) <= slack / 4, (r, ids, norm)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("arch", ARCHITECTURES)
 def test_bfloat16_search_from_graphs_is_the_one_launch_by_launch(tmp_path, arch):
