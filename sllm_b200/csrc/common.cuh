@@ -146,13 +146,14 @@ __device__ __forceinline__ float4 load_now_l2(const float4* p) {
 // Whether a launch on this stream may have the attribute: not where it is off, and not where the launch before made a step's description (lengths, block tables), which the attention
 // kernels read before their wait.  `pdl_description_made` says so behind such a launch; the next one of this library on the stream then begins when everything before it has completed and
 // is visible, and with it all that follow.
+bool pdl_enabled();
 bool pdl_allowed(cudaStream_t stream);
 void pdl_description_made(cudaStream_t stream);
 int num_sms();           // streaming multiprocessors of the current device (asked once per device)
 
 template <typename... KArgs, typename... Args>
-inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                          Args&&... args) {
+inline void launch_kernel_as(bool early, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                             Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -162,8 +163,20 @@ inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_allowed(stream) ? 1 : 0;
+  cfg.numAttrs = early ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);   // errors are read by launch_status()
+}
+template <typename... KArgs, typename... Args>
+inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                          Args&&... args) {
+  launch_kernel_as(pdl_allowed(stream), kernel, grid, block, smem, stream, static_cast<Args&&>(args)...);
+}
+// For the kernels that make a description, which read nothing before their wait: early themselves, also behind one another (2 us a launch otherwise), and what comes behind is not.
+template <typename... KArgs, typename... Args>
+inline void launch_kernel_describing(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                     Args&&... args) {
+  launch_kernel_as(pdl_enabled(), kernel, grid, block, smem, stream, static_cast<Args&&>(args)...);
+  pdl_description_made(stream);
 }
 
 // The shared memory that a kernel has been told it may use, a device each: the setting belongs to a device's copy of the kernel, and a process may hold models on

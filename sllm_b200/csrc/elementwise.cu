@@ -17,7 +17,7 @@ void set_error(const char* msg) {
   g_error[sizeof g_error - 1] = 0;
 }
 
-static bool pdl_enabled() {
+bool pdl_enabled() {
   static const bool on = [] {
     const char* v = getenv("SLLM_PDL");
     return !(v && v[0] == '0');

@@ -12,7 +12,7 @@
 // (a thousand lengths are four a thread; a launch of its own for them would cost more).  Measured, us: 8 decoded tokens 2.7, 48 requests with 4,099 tokens in two groups and new pages 6.6, 512 requests
 // with 32,768 tokens and tables of 2,100 columns 7.0 (1.0 for its bytes): the sums and the look-ups, one after the other, bound it.
 //
-// Attention kernels read lengths and block tables before they wait for the kernel before, so the launch behind either operator is a plain one (`pdl_description_made`).
+// Attention kernels read lengths and block tables before they wait for the kernel before, so the launch behind either operator is a plain one (`launch_kernel_describing`).
 #include "common.cuh"
 
 namespace sllm {
@@ -375,8 +375,7 @@ SLLM_EXPORT int sllm_beam_reorder(const int* parents, const int* slots, const in
   SLLM_REQUIRE(units * G * B < (1ll << 30), "beam_reorder: %lld bytes a beam", units * plan.unit);
   const long long work = units * G * B + (cells * G * B + 1023) / 1024, most = (long long)num_sms() * 4;
   const int grid = (int)(work < 1 ? 1 : work < most ? work : most);
-  launch_kernel(beam_reorder_kernel, grid, REORDER_THREADS, (size_t)(3 * G * B + 1) * sizeof(int), stream, parents, slots, lens, len_step, new_slots, G, B, plan);
-  pdl_description_made(stream);
+  launch_kernel_describing(beam_reorder_kernel, grid, REORDER_THREADS, (size_t)(3 * G * B + 1) * sizeof(int), stream, parents, slots, lens, len_step, new_slots, G, B, plan);
   return launch_status("beam_reorder");
 }
 
@@ -397,7 +396,6 @@ SLLM_EXPORT int sllm_step_tables(const int* q_lens, const int* have, const int* 
   }
   long long y = (most + TABLES_THREADS - 1) / TABLES_THREADS, room = 8ll * num_sms() / S;
   y = y < room ? y : room;
-  launch_kernel(step_tables_kernel, dim3((unsigned)S, (unsigned)(y < 1 ? 1 : y)), TABLES_THREADS, 0, stream, q_lens, have, rows, S, N, T, page_size, q_start, ctx_len, positions, seq_of_token, gs);
-  pdl_description_made(stream);
+  launch_kernel_describing(step_tables_kernel, dim3((unsigned)S, (unsigned)(y < 1 ? 1 : y)), TABLES_THREADS, 0, stream, q_lens, have, rows, S, N, T, page_size, q_start, ctx_len, positions, seq_of_token, gs);
   return launch_status("step_tables");
 }

@@ -2653,17 +2653,24 @@ def _typed(what: str, dtype, shape, *tensors) -> None:
 
 def _apart(what: str, written, read, own=()) -> None:
     """No tensor of ``written`` shares memory with another, or with one of ``read``.  ``own``: pairs (written, read) of which the one may be the whole other."""
-    same = {(id(w), id(r)) for w, r in own if w is not None and w.data_ptr() == r.data_ptr() and w.shape == r.shape}
-    gone = {r for _, r in same}
-    spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), True) for t in written if t is not None and t.numel()] +
-                   [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), False) for t in read if t is not None and t.numel() and id(t) not in gone])
+    gone = {id(r) for w, r in own if w.data_ptr() == r.data_ptr() and w.shape == r.shape}
+    spans = []
+    for t in written:
+        if t is not None and t.nbytes:
+            spans.append((t.data_ptr(), t.nbytes, True))
+    for t in read:
+        if t is not None and t.nbytes and id(t) not in gone:
+            spans.append((t.data_ptr(), t.nbytes, False))
+    spans.sort()
     end = end_written = 0
-    for first, last, is_written in spans:
+    for first, size, is_written in spans:
         if first < (end if is_written else end_written):
             raise KernelError(f"{what}: what is written cannot be what is read, nor lie over another result")
-        end = max(end, last)
-        if is_written:
-            end_written = max(end_written, last)
+        last = first + size
+        if last > end:
+            end = last
+        if is_written and last > end_written:
+            end_written = last
 
 
 @functools.lru_cache(maxsize=4096)
