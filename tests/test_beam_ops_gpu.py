@@ -115,6 +115,23 @@ def test_candidates_of_rows_of_huge_logits(V, dtype):
     _check_candidates(x.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype).reshape(-1, V).contiguous(), -torch.rand(len(sizes), 3, device=dev, generator=g), 6)
 
 
+@pytest.mark.parametrize("V", [900, 20011, 70001])
+@pytest.mark.parametrize("at", [2907270.0, -2907270.0, 0.0])
+def test_candidates_of_rows_across_a_border_of_the_sum(V, at):
+    """Logits around +-2^22 / log2 e, where a sum's reference is no whole number any longer, threads and parts of a row on either side of it; and rows with few logits of +-1e7 and 1e30 among
+    ordinary ones, early, late and everywhere."""
+    dev = cuda_or_skip()
+    g = torch.Generator(device=dev).manual_seed(V)
+    x = torch.randn(3, 4, V, device=dev, generator=g) * 2 + at
+    x[0, 0, : V // 2] -= 7
+    x[0, 1, V // 2 :] -= 7
+    x[0, 2] = x[0, 2].sort().values
+    if at == 0:
+        x[1, 0, 3], x[1, 1, V - 1], x[1, 2, V // 2], x[1, 3, ::7] = 1e7, 1e7, 1e30, 1e30
+        x[2, 0, : V - 3], x[2, 1, 3:], x[2, 2, ::2], x[2, 3, 1::2] = -1e7, -1e7, -1e30, -3e6
+    _check_candidates(x.reshape(12, V), -torch.rand(3, 4, device=dev, generator=g), 5)
+
+
 @pytest.mark.parametrize("V", [40, 3001, 50000])
 @pytest.mark.parametrize("keep", [1, 2, 3, 9])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
