@@ -111,7 +111,8 @@ attention_tma_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __g
   }
   __syncthreads();
   // The batch description (tiles, lengths, block tables) was copied to the device before the step's
-  // first kernel started, so it is read before the wait for the step's earlier kernels: the chain of
+  // first kernel started, or made by kernels that the launch behind them waited for
+  // (launch_kernel_describing), so it is read before the wait for the step's earlier kernels: the chain of
   // dependent loads (tile -> request -> lengths -> pages) runs under their tails.  The queries and the
   // new keys and values come from those kernels: each role waits before it touches them.
 

@@ -10,8 +10,8 @@
 // Exponentials and a batch's sum of them (16 terms) are float32; the sums over batches, threads and parts, the logarithm and s are of 48 bits and more, because continuations of different beams
 // are compared with each other (those of one beam by their logits alone).  Where two beams' lie closer than those float32 steps can tell, their sums are made again in float64 (see `beam_close`).
 // s is rounded to float32 once, when it is stored.
-// Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 10.8 (0.4), 35 of 32,001 13.9 (0.7), 512 of 152,064 float32 63 (47.6) and
-// bfloat16 54.5 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
+// Measured, both kernels, us (reading the logits at the measured copy rate): 4 rows of 151,936 float32 10.3 (0.4), 35 of 32,001 13.3 (0.7), 512 of 152,064 float32 63 (47.6) and
+// bfloat16 53.6 (23.8).  Few rows are bound by the chain load, first bound, list, sums, join, about a microsecond each; many by HBM through the long runs, and by the same chain, which their blocks go
 // through side by side.
 #include <float.h>
 
